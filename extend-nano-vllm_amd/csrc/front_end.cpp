@@ -95,6 +95,11 @@ at::Tensor empty_bf16(at::IntArrayRef sizes, const at::Tensor& like) {
   return at::empty(sizes, at::TensorOptions().dtype(at::kBFloat16).device(like.device()));
 }
 
+at::Tensor empty_bytes(size_t bytes, const at::Tensor& like) {
+  return at::empty({static_cast<int64_t>(bytes)},
+                   at::TensorOptions().dtype(at::kByte).device(like.device()));
+}
+
 // The current stream of the current device, as the Python path takes it;
 // `only` >= 0 leaves another current device to the general path.
 void* current_stream(int64_t only = -1) {
@@ -479,6 +484,194 @@ PyObject* linear(PyObject*, PyObject* const* v, Py_ssize_t n) {
   });
 }
 
+// (q, k_cache, v_cache, cu_q, cu_k, max_q, max_k, prefix_len, softmax_scale, block_table,
+//  k_scale | None, v_scale | None, out | None) -> out
+PyObject* shared_prefix_attention_varlen(PyObject*, PyObject* const* v, Py_ssize_t n) {
+  return guarded(n, 13, [&]() -> PyObject* {
+    Args a{v};
+    const at::Tensor& q = a.tensor(0);
+    const at::Tensor& cu_q = a.tensor(3);
+    const at::Tensor& cu_k = a.tensor(4);
+    const at::Tensor& bt = a.tensor(9);
+    const int32_t max_q = a.i32(5), max_k = a.i32(6), prefix = a.i32(7);
+    const float scale = a.f32(8);
+    const float* ks = a.scale(10);
+    const float* vs = a.scale(11);
+    need_i32(cu_q);
+    need_i32(cu_k);
+    const int32_t b = as_i32(cu_q.numel() - 1);
+    const Attention r = attention(a, q, 1, 2, bt, 12);
+    need(b > 0 && cu_k.numel() == b + 1 && bt.size(0) >= b && r.t > 0 && r.hq > 0);
+    need(prefix >= 0 && prefix <= int64_t{r.bt_cols} * r.p.block_size);
+    void* s = current_stream(a.device);
+    const size_t bytes =
+        nva_shared_prefix_workspace_size(b, r.t, r.hq, r.p.hkv, r.p.d, max_q, max_k, prefix);
+    need(bytes > 0);
+    const at::Tensor w = empty_bytes(bytes, q);
+    launch([&] {
+      return nva_shared_prefix_attention_varlen(
+          q.data_ptr(), q.stride(0), q.stride(1), r.p.k, r.p.v, r.p.kv_dtype, r.p.blk, r.p.tok,
+          r.p.head, r.p.num_blocks, r.p.block_size, static_cast<const int32_t*>(cu_q.data_ptr()),
+          static_cast<const int32_t*>(cu_k.data_ptr()), static_cast<const int32_t*>(bt.data_ptr()),
+          bt.stride(0), r.bt_cols, b, r.t, max_q, max_k, prefix, r.hq, r.p.hkv, r.p.d, scale, ks, vs,
+          r.out.data_ptr(), r.out.stride(0), r.out.stride(1), w.data_ptr(), bytes, s);
+    });
+    return THPVariable_Wrap(r.out);
+  });
+}
+
+// (q, k_cache, v_cache, cache_seqlens, block_table, prefix_len, softmax_scale, max_k | None,
+//  k_scale | None, v_scale | None, out | None) -> out
+PyObject* shared_prefix_attention_decode(PyObject*, PyObject* const* v, Py_ssize_t n) {
+  return guarded(n, 11, [&]() -> PyObject* {
+    Args a{v};
+    const at::Tensor& q = a.tensor(0);
+    const at::Tensor& lens = a.tensor(3);
+    const at::Tensor& bt = a.tensor(4);
+    const int32_t prefix = a.i32(5);
+    const float scale = a.f32(6);
+    const float* ks = a.scale(8);
+    const float* vs = a.scale(9);
+    need_i32(lens);
+    const Attention r = attention(a, q, 1, 2, bt, 10);
+    need(lens.numel() == r.t && bt.size(0) >= r.t && r.t > 0 && r.hq > 0);
+    const int32_t all = as_i32(int64_t{r.bt_cols} * r.p.block_size);
+    const int32_t max_k = a.none(7) ? all : a.i32(7);
+    need(prefix >= 0 && prefix <= all);
+    void* s = current_stream(a.device);
+    const size_t bytes =
+        nva_shared_prefix_workspace_size(r.t, r.t, r.hq, r.p.hkv, r.p.d, 1, max_k, prefix);
+    need(bytes > 0);
+    const at::Tensor w = empty_bytes(bytes, q);
+    launch([&] {
+      return nva_shared_prefix_attention_decode(
+          q.data_ptr(), q.stride(0), q.stride(1), r.p.k, r.p.v, r.p.kv_dtype, r.p.blk, r.p.tok,
+          r.p.head, r.p.num_blocks, r.p.block_size, static_cast<const int32_t*>(lens.data_ptr()),
+          static_cast<const int32_t*>(bt.data_ptr()), bt.stride(0), r.bt_cols, r.t, max_k, prefix,
+          r.hq, r.p.hkv, r.p.d, scale, ks, vs, r.out.data_ptr(), r.out.stride(0), r.out.stride(1),
+          w.data_ptr(), bytes, s);
+    });
+    return THPVariable_Wrap(r.out);
+  });
+}
+
+bool wants_grad(const at::Tensor& t) { return at::GradMode::is_enabled() && t.requires_grad(); }
+
+// (x, qweight, scales, zeros | None, bias | None, out | None) -> out
+PyObject* linear_w4(PyObject*, PyObject* const* v, Py_ssize_t n) {
+  return guarded(n, 6, [&]() -> PyObject* {
+    Args a{v};
+    const at::Tensor& x = a.tensor(0);
+    const at::Tensor& w = a.tensor(1);
+    const at::Tensor& sc = a.tensor(2);
+    need_rows(x);
+    need(w.scalar_type() == at::kByte && w.dim() == 2 && w.is_contiguous());
+    need(sc.scalar_type() == at::kBFloat16 && sc.dim() == 2 && sc.is_contiguous());
+    need(!wants_grad(x) && !wants_grad(sc));
+    const int32_t rows = as_i32(x.size(0)), k = as_i32(x.size(1)), m = as_i32(w.size(0));
+    need(rows > 0 && k > 0 && m > 0 && k % 2 == 0 && w.size(1) == k / 2 && sc.size(1) == m &&
+         sc.size(0) > 0 && k % sc.size(0) == 0);
+    const int32_t group = static_cast<int32_t>(k / sc.size(0));
+    const void* zeros = nullptr;
+    if (!a.none(3)) {
+      const at::Tensor& z = a.tensor(3);
+      need(z.scalar_type() == at::kByte && z.is_contiguous() && z.sizes() == sc.sizes());
+      zeros = z.data_ptr();
+    }
+    const void* bias = nullptr;
+    if (!a.none(4)) {
+      const at::Tensor& b = a.tensor(4);
+      need(b.scalar_type() == at::kBFloat16 && b.dim() == 1 && b.is_contiguous() && b.size(0) == m &&
+           !wants_grad(b));
+      bias = b.data_ptr();
+    }
+    need(x.stride(0) >= k && x.stride(0) % 8 == 0 && reinterpret_cast<uintptr_t>(x.data_ptr()) % 16 == 0);
+    at::Tensor out;
+    if (a.none(5)) {
+      out = empty_bf16({rows, m}, x);
+    } else {
+      out = a.tensor(5);
+      need_rows(out);
+      need(out.size(0) == rows && out.size(1) == m && out.stride(0) >= m);
+    }
+    void* s = current_stream(a.device);
+    launch([&] {
+      return nva_linear_w4(x.data_ptr(), x.stride(0), w.data_ptr(), sc.data_ptr(), zeros, bias,
+                           out.data_ptr(), out.stride(0), rows, m, k, group, s);
+    });
+    return THPVariable_Wrap(out);
+  });
+}
+
+// (positions, q, k | None, inv_freq, interleaved, factor, q_out | None, k_out | None) ->
+// (q_out, k_out | None): new outputs, or in place
+PyObject* rotary_embedding(PyObject*, PyObject* const* v, Py_ssize_t n) {
+  return guarded(n, 8, [&]() -> PyObject* {
+    Args a{v};
+    const at::Tensor& pos = a.tensor(0);
+    const at::Tensor& q = a.tensor(1);
+    const at::Tensor& freq = a.tensor(3);
+    need(PyBool_Check(v[4]));
+    const bool interleaved = v[4] == Py_True;
+    const float factor = a.f32(5);
+    const bool has_k = !a.none(2);
+    const at::Tensor& k = has_k ? a.tensor(2) : q;
+    int dtype = 0;
+    switch (q.scalar_type()) {
+      case at::kBFloat16: dtype = NVA_BF16; break;
+      case at::kHalf: dtype = NVA_F16; break;
+      case at::kFloat: dtype = NVA_F32; break;
+      default: throw Other{};
+    }
+    need(q.dim() == 3 && q.stride(2) == 1 && k.dim() == 3 && k.stride(2) == 1 &&
+         k.scalar_type() == q.scalar_type() && k.size(0) == q.size(0) && k.size(2) == q.size(2));
+    need(!wants_grad(q) && !wants_grad(k) && !wants_grad(freq));
+    const int32_t t = as_i32(q.size(0)), hq = as_i32(q.size(1)), hk = as_i32(k.size(1)),
+                  d = as_i32(q.size(2));
+    need(pos.scalar_type() == at::kLong && pos.is_contiguous() && pos.numel() == t);
+    need(freq.scalar_type() == at::kDouble && freq.dim() == 1 && freq.is_contiguous() &&
+         freq.size(0) > 0 && 2 * freq.size(0) <= d);
+    at::Tensor q_out, k_out;
+    if (a.none(6) && a.none(7)) {
+      const auto options = at::TensorOptions().dtype(q.dtype()).device(q.device());
+      q_out = at::empty(q.sizes(), options);
+      if (has_k) k_out = at::empty(k.sizes(), options);
+    } else {
+      // in place: heads that do not overlap, and q and k in different columns of
+      // the same rows
+      need(v[6] == v[1] && v[7] == v[2] && t > 0 && hq > 0 && hk > 0);
+      const int64_t size = q.element_size();
+      const int64_t row = q.stride(0), wq = (hq - 1) * q.stride(1) + d, wk = (hk - 1) * k.stride(1) + d;
+      need(q.stride(1) >= d && row >= wq);
+      if (has_k) {
+        const int64_t bytes = static_cast<char*>(k.data_ptr()) - static_cast<char*>(q.data_ptr());
+        need(k.stride(1) >= d && k.stride(0) == row && bytes % size == 0);
+        int64_t at = bytes / size % row;
+        if (at < 0) at += row;
+        need(at >= wq && at + wk <= row);
+      }
+      q_out = q;
+      if (has_k) k_out = k;
+    }
+    void* s = current_stream(a.device);
+    launch([&] {
+      return nva_rotary_embedding(
+          static_cast<const int64_t*>(pos.data_ptr()), static_cast<const double*>(freq.data_ptr()),
+          factor, interleaved, dtype, q.data_ptr(), q.stride(0), q.stride(1), hq,
+          has_k ? k.data_ptr() : nullptr, has_k ? k.stride(0) : 0, has_k ? k.stride(1) : 0,
+          has_k ? hk : 0, t, d, as_i32(2 * freq.size(0)), q_out.data_ptr(), q_out.stride(0),
+          q_out.stride(1), has_k ? k_out.data_ptr() : nullptr, has_k ? k_out.stride(0) : 0,
+          has_k ? k_out.stride(1) : 0, s);
+    });
+    PyObject* first = THPVariable_Wrap(q_out);
+    PyObject* second = has_k ? THPVariable_Wrap(k_out) : Py_NewRef(Py_None);
+    PyObject* both = PyTuple_Pack(2, first, second);
+    Py_XDECREF(first);
+    Py_XDECREF(second);
+    return both;
+  });
+}
+
 // (x [T, H, D]) -> its view [T, H * D]
 PyObject* merge_heads(PyObject*, PyObject* const* v, Py_ssize_t n) {
   return guarded(n, 1, [&]() -> PyObject* {
@@ -508,6 +701,10 @@ PyMethodDef methods[] = {
     FAST("paged_attention_decode", paged_attention_decode),
     FAST("argmax_rows", argmax_rows),
     FAST("linear", linear),
+    FAST("linear_w4", linear_w4),
+    FAST("rotary_embedding", rotary_embedding),
+    FAST("shared_prefix_attention_varlen", shared_prefix_attention_varlen),
+    FAST("shared_prefix_attention_decode", shared_prefix_attention_decode),
     FAST("merge_heads", merge_heads),
     FAST("place", place),
     {nullptr, nullptr, 0, nullptr},

@@ -30,6 +30,10 @@ ARGMAX_STATIC_KEYS = 65536      # NVA_ARGMAX_STATIC_KEYS of the header
 KV_BF16 = 0
 KV_FP8_E4M3 = 1
 
+DTYPE_BF16 = 0
+DTYPE_F16 = 1
+DTYPE_F32 = 2
+
 # Every symbol the header declares, with (restype, argtypes).
 _P = ctypes.c_void_p
 _I32 = ctypes.c_int32
@@ -70,6 +74,18 @@ SIGNATURES = {
     "nva_silu_mul": (_INT, [_P, _I64, _P, _I64, _I32, _I32, _P]),
     "nva_linear_preferred": (_INT, [_I32, _I32, _I32]),
     "nva_linear": (_INT, [_P, _I64, _P, _P, _I64, _I32, _I32, _I32, _P]),
+    "nva_linear_w4": (_INT, [_P, _I64, _P, _P, _P, _P, _P, _I64, _I32, _I32, _I32, _I32, _P]),
+    "nva_rotary_embedding": (_INT, [_P, _P, _F32, _INT, _INT, _P, _I64, _I64, _I32, _P, _I64, _I64,
+                                    _I32, _I32, _I32, _I32, _P, _I64, _I64, _P, _I64, _I64, _P]),
+    "nva_shared_prefix_workspace_size": (_SZ, [_I32, _I32, _I32, _I32, _I32, _I32, _I32, _I32]),
+    "nva_shared_prefix_attention_varlen": (_INT, [_P, _I64, _I64, _P, _P, _INT, _I64, _I64, _I64,
+                                                  _I32, _I32, _P, _P, _P, _I64, _I32, _I32, _I32,
+                                                  _I32, _I32, _I32, _I32, _I32, _I32, _F32, _P, _P,
+                                                  _P, _I64, _I64, _P, _SZ, _P]),
+    "nva_shared_prefix_attention_decode": (_INT, [_P, _I64, _I64, _P, _P, _INT, _I64, _I64, _I64,
+                                                  _I32, _I32, _P, _P, _I64, _I32, _I32, _I32, _I32,
+                                                  _I32, _I32, _I32, _F32, _P, _P, _P, _I64, _I64,
+                                                  _P, _SZ, _P]),
     "nva_verify_metadata": (_INT, [_P, _P, _I32, _P, _I64, _I32, _I32, _P, _P, _P, _P, _I32, _P]),
     "nva_draft_metadata": (_INT, [_P, _P, _P, _I32, _I32, _I32, _P, _I64, _I32, _I32, _I32, _P,
                                   _P, _P, _P]),

@@ -520,6 +520,134 @@ def paged_attention_decode(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torc
     return out
 
 
+def shared_prefix_workspace_bytes(num_seqs: int, num_tokens: int, num_q_heads: int,
+                                  num_kv_heads: int, head_dim: int, max_seqlen_q: int,
+                                  max_seqlen_k: int, prefix_len: int) -> int:
+    return int(_native.load().nva_shared_prefix_workspace_size(
+        num_seqs, num_tokens, num_q_heads, num_kv_heads, head_dim, max_seqlen_q, max_seqlen_k,
+        prefix_len))
+
+
+def _prefix_args(q, k_cache, v_cache, block_table, num_seqs: int, prefix_len: int, max_k: int,
+                 out, scale: float):
+    """The checks that the two shared-prefix entry points have in common:
+    cache arguments, output, and the prefix against the table."""
+    cache = _cache_args(k_cache, v_cache)
+    bs, hkv, d = cache[5:]
+    if q.dim() != 3 or q.shape[2] != d:
+        raise ValueError("q must be [tokens, num_heads, head_dim] with the cache's head_dim")
+    if hkv == 0 or q.shape[1] % hkv != 0:
+        raise ValueError("num query heads must divide evenly by KV heads")
+    if block_table.dtype != torch.int32 or block_table.dim() != 2 or block_table.stride(1) != 1:
+        raise TypeError("block_table must be int32 [num_seqs, max_blocks]")
+    if block_table.shape[0] < num_seqs:
+        raise ValueError("block_table must have one row per sequence")
+    if not 0 <= prefix_len <= block_table.shape[1] * bs:
+        raise ValueError("prefix_len must be within the keys that a block_table row can list")
+    if max_k < 0:
+        raise ValueError("max_seqlen_k must not be negative")
+    if not scale > 0:
+        raise ValueError("softmax_scale must be positive")
+    return cache, _q_out(q, out)
+
+
+def shared_prefix_attention_varlen(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor,
+                                   cu_seqlens_q: torch.Tensor, cu_seqlens_k: torch.Tensor,
+                                   max_seqlen_q: int, max_seqlen_k: int, prefix_len: int,
+                                   softmax_scale: float, block_table: torch.Tensor,
+                                   k_scale: torch.Tensor | None = None,
+                                   v_scale: torch.Tensor | None = None,
+                                   out: torch.Tensor | None = None) -> torch.Tensor:
+    """``paged_attention_varlen`` of a batch whose sequences share their first
+    ``prefix_len`` keys, which are read once for the whole batch.
+
+    The result is paged_attention_varlen's.  Every sequence's first prefix_len
+    keys must be those that row 0 of ``block_table`` lists: the same pages (the
+    prefix cache shares whole ones), or copies of them.  Row 0 lists the whole
+    prefix whatever sequence 0's length; a shorter sequence sees its own length
+    of it.  Rows of no sequence are left as they are."""
+    got = (_front or _front_end()).shared_prefix_attention_varlen(
+        q, k_cache, v_cache, cu_seqlens_q, cu_seqlens_k, max_seqlen_q, max_seqlen_k, prefix_len,
+        softmax_scale, block_table, k_scale, v_scale, out)
+    if got is not None:
+        return got
+    lib = _native.load()
+    _require_cuda(q, k_cache, v_cache, block_table, out, _scale(k_scale), _scale(v_scale))
+    cu_seqlens_q, host_q = _device_lengths(cu_seqlens_q, q.device, "cu_seqlens_q")
+    cu_seqlens_k, host_k = _device_lengths(cu_seqlens_k, q.device, "cu_seqlens_k")
+    if host_q is not None:
+        _check_bound(int(max_seqlen_q), [b - a for a, b in zip(host_q, host_q[1:])],
+                     "query length", "max_seqlen_q")
+    if host_k is not None:
+        _check_bound(int(max_seqlen_k), [b - a for a, b in zip(host_k, host_k[1:])],
+                     "key length", "max_seqlen_k")
+    _i32(cu_seqlens_q, "cu_seqlens_q")
+    _i32(cu_seqlens_k, "cu_seqlens_k")
+    b = cu_seqlens_q.numel() - 1
+    if b < 0 or cu_seqlens_k.numel() != b + 1:
+        raise ValueError("cu_seqlens_k does not match cu_seqlens_q")
+    (kvd, bstr, tstr, hstr, nb, bs, hkv, d), out = _prefix_args(
+        q, k_cache, v_cache, block_table, b, int(prefix_len), int(max_seqlen_k), out,
+        float(softmax_scale))
+    t, hq, _ = q.shape
+    with torch.cuda.device(q.device):
+        nbytes = shared_prefix_workspace_bytes(b, t, hq, hkv, d, int(max_seqlen_q),
+                                               int(max_seqlen_k), int(prefix_len))
+        ws = torch.empty(nbytes, dtype=torch.uint8, device=q.device)
+        check(lib.nva_shared_prefix_attention_varlen(
+            q.data_ptr(), q.stride(0), q.stride(1), k_cache.data_ptr(), v_cache.data_ptr(), kvd,
+            bstr, tstr, hstr, nb, bs, cu_seqlens_q.data_ptr(), cu_seqlens_k.data_ptr(),
+            block_table.data_ptr(), block_table.stride(0), block_table.shape[1], b, t,
+            int(max_seqlen_q), int(max_seqlen_k), int(prefix_len), hq, hkv, d,
+            float(softmax_scale), _ptr(k_scale), _ptr(v_scale), out.data_ptr(), out.stride(0),
+            out.stride(1), ws.data_ptr(), nbytes, _stream()), "shared_prefix_attention_varlen")
+    return out
+
+
+def shared_prefix_attention_decode(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor,
+                                   cache_seqlens: torch.Tensor, block_table: torch.Tensor,
+                                   prefix_len: int, softmax_scale: float,
+                                   max_seqlen_k: int | None = None,
+                                   k_scale: torch.Tensor | None = None,
+                                   v_scale: torch.Tensor | None = None,
+                                   out: torch.Tensor | None = None) -> torch.Tensor:
+    """``paged_attention_decode`` (one query row per sequence) of a batch whose
+    sequences share their first ``prefix_len`` keys; see
+    ``shared_prefix_attention_varlen``."""
+    got = (_front or _front_end()).shared_prefix_attention_decode(
+        q, k_cache, v_cache, cache_seqlens, block_table, prefix_len, softmax_scale, max_seqlen_k,
+        k_scale, v_scale, out)
+    if got is not None:
+        return got
+    lib = _native.load()
+    _require_cuda(q, k_cache, v_cache, block_table, out, _scale(k_scale), _scale(v_scale))
+    cache_seqlens, host_lens = _device_lengths(cache_seqlens, q.device, "cache_seqlens")
+    _i32(cache_seqlens, "cache_seqlens")
+    b = q.shape[0]
+    if cache_seqlens.numel() != b:
+        raise ValueError("cache_seqlens must have one entry per query")
+    if max_seqlen_k is None:
+        max_seqlen_k = block_table.shape[-1] * k_cache.shape[1]
+    if host_lens is not None:
+        _check_bound(int(max_seqlen_k), host_lens, "context length", "max_seqlen_k")
+    (kvd, bstr, tstr, hstr, nb, bs, hkv, d), out = _prefix_args(
+        q, k_cache, v_cache, block_table, b, int(prefix_len), int(max_seqlen_k), out,
+        float(softmax_scale))
+    hq = q.shape[1]
+    with torch.cuda.device(q.device):
+        nbytes = shared_prefix_workspace_bytes(b, b, hq, hkv, d, 1, int(max_seqlen_k),
+                                               int(prefix_len))
+        ws = torch.empty(nbytes, dtype=torch.uint8, device=q.device)
+        check(lib.nva_shared_prefix_attention_decode(
+            q.data_ptr(), q.stride(0), q.stride(1), k_cache.data_ptr(), v_cache.data_ptr(), kvd,
+            bstr, tstr, hstr, nb, bs, cache_seqlens.data_ptr(), block_table.data_ptr(),
+            block_table.stride(0), block_table.shape[1], b, int(max_seqlen_k), int(prefix_len), hq,
+            hkv, d, float(softmax_scale), _ptr(k_scale), _ptr(v_scale), out.data_ptr(),
+            out.stride(0), out.stride(1), ws.data_ptr(), nbytes, _stream()),
+            "shared_prefix_attention_decode")
+    return out
+
+
 def fp8_paged_decode_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor,
                                context_lens: torch.Tensor, block_tables: torch.Tensor,
                                scale: float, k_scale: torch.Tensor,
@@ -697,6 +825,202 @@ def linear(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | None = No
     library."""
     got = (_front or _front_end()).linear(x, weight, bias)
     return torch.nn.functional.linear(x, weight, bias) if got is None else got
+
+
+def _no_grad(name: str, *tensors: torch.Tensor) -> None:
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
+        raise ValueError(f"{name} computes no gradients: call it under torch.no_grad()")
+
+
+def quantize_w4(weight: torch.Tensor, group_size: int = 128, zeros: bool = False):
+    """4-bit codes and group scales of a weight [n, k], as ``linear_w4`` takes
+    them: (qweight uint8 [n, k / 2], scales bf16 [k / group_size, n], zeros uint8
+    [k / group_size, n] or None).
+
+    Rounds each weight to the nearest of 16 levels of its group: without zeros
+    -8 .. 7 times the scale, the largest magnitude at 7 or at -8, whichever
+    leaves the smaller scale; with zeros from the group's least value (or 0) to
+    its greatest (or 0).  Scales are rounded to bf16 before the codes are
+    formed, so the codes are the nearest for the scale that is used."""
+    if weight.dim() != 2 or not weight.is_floating_point():
+        raise ValueError("weight must be a floating-point [n, k]")
+    n, k = weight.shape
+    if group_size < 32 or group_size % 32 or k == 0 or k % group_size:
+        raise ValueError("group_size must be a multiple of 32 that divides k")
+    with torch.no_grad():
+        w = weight.float().view(n, k // group_size, group_size)
+        lo, hi = w.amin(-1), w.amax(-1)
+        if zeros:
+            lo, hi = lo.clamp(max=0.0), hi.clamp(min=0.0)
+            scales = ((hi - lo) / 15).to(BF16)
+            step = torch.where(scales > 0, scales.float(), 1.0)
+            zero = (-lo / step).round().clamp(0, 15)
+        else:
+            scales = torch.maximum(-lo / 8, hi / 7).clamp(min=0.0).to(BF16)
+            step = torch.where(scales > 0, scales.float(), 1.0)
+            zero = torch.full_like(step, 8.0)
+        codes = ((w / step[..., None]).round() + zero[..., None]).clamp(0, 15).to(torch.uint8)
+        codes = codes.view(n, k)
+        return (codes[:, 0::2] | (codes[:, 1::2] << 4), scales.t().contiguous(),
+                zero.t().to(torch.uint8).contiguous() if zeros else None)
+
+
+def linear_w4(x: torch.Tensor, qweight: torch.Tensor, scales: torch.Tensor,
+              zeros: torch.Tensor | None = None, bias: torch.Tensor | None = None,
+              out: torch.Tensor | None = None) -> torch.Tensor:
+    """``linear`` over 4-bit weights with group scales.
+
+    out[m, j] = sum_i x[m, i] (code[j, i] - zero[i / G, j]) scale[i / G, j] + bias[j],
+    G = k / scales.shape[0], in float32, rounded to bf16 once (no weight is
+    rounded).  x: bf16 [rows, k]; qweight: uint8 [n, k / 2], element 2 i in the
+    low half of byte i; scales: bf16 [k / G, n]; zeros: uint8 [k / G, n] of 0..15,
+    None for 8; bias: bf16 [n].  G is a multiple of 32.  Made for up to 64 rows
+    (a step's tokens); more rows run 64 at a time.  A row of x that holds an
+    infinity or a NaN comes out NaN."""
+    got = (_front or _front_end()).linear_w4(x, qweight, scales, zeros, bias, out)
+    if got is not None:
+        return got
+    lib = _native.load()
+    _require_cuda(x, qweight, scales, zeros, bias, out)
+    _no_grad("linear_w4", x, scales, bias)
+    if x.dtype != BF16 or x.dim() != 2:
+        raise ValueError("x must be bf16 [rows, k]")
+    rows, k = x.shape
+    if qweight.dtype != torch.uint8 or qweight.dim() != 2 or not qweight.is_contiguous() \
+            or k == 0 or k % 2 or qweight.shape[1] != k // 2:
+        raise ValueError("qweight must be contiguous uint8 [n, k / 2]")
+    n = qweight.shape[0]
+    if scales.dtype != BF16 or scales.dim() != 2 or not scales.is_contiguous() \
+            or scales.shape[0] == 0 or scales.shape[1] != n or k % scales.shape[0]:
+        raise ValueError("scales must be contiguous bf16 [k / group, n]")
+    group = k // scales.shape[0]
+    if group % 32:
+        raise ValueError("the group size must be a multiple of 32")
+    if zeros is not None and (zeros.dtype != torch.uint8 or zeros.shape != scales.shape
+                              or not zeros.is_contiguous()):
+        raise ValueError("zeros must be contiguous uint8 [k / group, n]")
+    if bias is not None and (bias.dtype != BF16 or bias.shape != (n,) or not bias.is_contiguous()):
+        raise ValueError("bias must be contiguous bf16 [n]")
+    if out is None:
+        out = torch.empty(rows, n, dtype=BF16, device=x.device)
+    elif out.dtype != BF16 or tuple(out.shape) != (rows, n) or out.stride(1) != 1:
+        raise ValueError("out must be bf16 [rows, n] with unit last stride")
+    if n == 0 or rows == 0:
+        return out
+    # the kernel reads x 16 bytes at a time
+    if x.stride(1) != 1 or (rows > 1 and (x.stride(0) % 8 or x.stride(0) < k)) \
+            or x.data_ptr() % 16:
+        x = x.clone(memory_format=torch.contiguous_format)
+    if rows > 1 and out.stride(0) < n:
+        raise ValueError("out rows must not overlap")
+    with torch.cuda.device(x.device):
+        check(lib.nva_linear_w4(x.data_ptr(), x.stride(0) if rows > 1 else k, qweight.data_ptr(),
+                                scales.data_ptr(), _ptr(zeros), _ptr(bias), out.data_ptr(),
+                                out.stride(0), rows, n, k, group, _stream()), "linear_w4")
+    return out
+
+
+_ROTARY_DTYPES = {BF16: _native.DTYPE_BF16, torch.float16: _native.DTYPE_F16,
+                  torch.float32: _native.DTYPE_F32}
+
+
+def _meet(a: torch.Tensor, b: torch.Tensor) -> bool:
+    """Whether two [T, H, D] tensors of one type may share an element: their
+    address ranges meet, and they are not different columns of rows of one
+    stride (the heads of a fused projection)."""
+    if a.numel() == 0 or b.numel() == 0:
+        return False
+    size = a.element_size()
+    spans = [sum((n - 1) * st for n, st in zip(x.shape, x.stride())) + 1 for x in (a, b)]
+    delta = (b.data_ptr() - a.data_ptr()) // size
+    if delta >= spans[0] or -delta >= spans[1]:
+        return False
+    row = a.stride(0)
+    if a.shape[0] > 1 and row == b.stride(0) and (b.data_ptr() - a.data_ptr()) % size == 0:
+        wa, wb = ((x.shape[1] - 1) * x.stride(1) + x.shape[2] for x in (a, b))
+        at = delta % row if row else 0
+        return at < wa or at + wb > row
+    return True
+
+
+def _self_overlap(x: torch.Tensor) -> bool:
+    covered = 1
+    for st, n in sorted((st, n) for st, n in zip(x.stride(), x.shape) if n > 1):
+        if st < covered:
+            return True
+        covered += st * (n - 1)
+    return False
+
+
+def rotary_embedding(positions: torch.Tensor, q: torch.Tensor, k: torch.Tensor | None,
+                     inv_freq: torch.Tensor, interleaved: bool = False, factor: float = 1.0,
+                     q_out: torch.Tensor | None = None, k_out: torch.Tensor | None = None):
+    """Rotary positions of query and key heads (layers/rotary_embedding.py:6-48,
+    in both layouts, over part of a head, at any frequencies).
+
+    Pair e of the head at position p turns by p * inv_freq[e] and is scaled by
+    ``factor``: elements e and e + rot / 2 of the head, or with ``interleaved``
+    2 e and 2 e + 1, rot = 2 * len(inv_freq); what follows the first rot
+    elements is copied.  Angles are formed in float64 (inv_freq is float64, see
+    ``layers.rope_frequencies``), the rest in float32 with one rounding.
+
+    q [T, Hq, D] and k [T, Hk, D] (or None): bf16, float16 or float32, any row and
+    head strides; positions int64 [T].  Returns (q_out, k_out), new contiguous
+    tensors unless given; q_out / k_out may be q / k themselves."""
+    got = (_front or _front_end()).rotary_embedding(positions, q, k, inv_freq, interleaved, factor,
+                                                    q_out, k_out)
+    if got is not None:
+        return got
+    lib = _native.load()
+    _require_cuda(positions, q, k, inv_freq, q_out, k_out)
+    _no_grad("rotary_embedding", q, k, inv_freq)
+    if q.dtype not in _ROTARY_DTYPES or q.dim() != 3:
+        raise ValueError("q must be bf16, float16 or float32 [tokens, heads, head_dim]")
+    t, hq, d = q.shape
+    if positions.dtype != torch.int64 or not positions.is_contiguous() or positions.numel() != t:
+        raise ValueError("positions must be contiguous int64 with one entry per token")
+    if k is not None and (k.dtype != q.dtype or k.dim() != 3 or k.shape[0] != t or k.shape[2] != d):
+        raise ValueError("k must be [tokens, heads, head_dim] like q")
+    if inv_freq.dtype != torch.float64 or inv_freq.dim() != 1 or not inv_freq.is_contiguous() \
+            or not 0 < 2 * inv_freq.numel() <= d:
+        raise ValueError("inv_freq must be contiguous float64 [rot / 2] with rot <= head_dim")
+    if k is None and k_out is not None:
+        raise ValueError("k_out without k")
+    outs = []
+    for x, out, name in ((q, q_out, "q"), (k, k_out, "k")):
+        if x is None:
+            outs.append(None)
+            continue
+        if x.stride(2) != 1:
+            raise ValueError(f"{name} must have unit stride over head_dim")
+        if out is None:
+            out = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+        elif out.dtype != x.dtype or out.shape != x.shape or out.stride(2) != 1:
+            raise ValueError(f"{name}_out must match {name} with unit stride over head_dim")
+        elif _self_overlap(out):
+            raise ValueError(f"{name}_out must not overlap itself")
+        outs.append(out)
+    # an output may be its input and meet no tensor otherwise: workgroups run
+    # in any order
+    for i, out in enumerate(outs):
+        for j, x in enumerate((q, k)):
+            if out is None or x is None:
+                continue
+            same = i == j and out.data_ptr() == x.data_ptr() and out.stride() == x.stride()
+            if not same and _meet(out, x):
+                raise ValueError("outputs may be their inputs and must not overlap them otherwise")
+    if outs[1] is not None and _meet(outs[0], outs[1]):
+        raise ValueError("q_out and k_out must not overlap")
+    k_args = (0, 0, 0, 0) if k is None else (k.data_ptr(), k.stride(0), k.stride(1), k.shape[1])
+    k_out_args = (0, 0, 0) if k is None else (outs[1].data_ptr(), outs[1].stride(0),
+                                              outs[1].stride(1))
+    with torch.cuda.device(q.device):
+        check(lib.nva_rotary_embedding(
+            positions.data_ptr(), inv_freq.data_ptr(), float(factor), int(bool(interleaved)),
+            _ROTARY_DTYPES[q.dtype], q.data_ptr(), q.stride(0), q.stride(1), hq, *k_args, t, d,
+            2 * inv_freq.numel(), outs[0].data_ptr(), outs[0].stride(0), outs[0].stride(1),
+            *k_out_args, _stream()), "rotary_embedding")
+    return tuple(outs)
 
 
 def silu_mul(x: torch.Tensor) -> torch.Tensor:

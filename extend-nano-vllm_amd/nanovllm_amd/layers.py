@@ -7,6 +7,7 @@ load unchanged.
 """
 from __future__ import annotations
 
+import math
 from functools import lru_cache
 
 import torch
@@ -86,6 +87,86 @@ def rope_cos_sin(head_dim: int, max_position: int, base: float, device_index: in
     freqs = torch.outer(t, inv_freq)
     table = torch.cat((freqs.cos(), freqs.sin()), dim=-1).contiguous()
     return table.to(torch.device("cuda", device_index))
+
+
+def rope_frequencies(rotary_dim: int, base: float, scaling: dict | None = None,
+                     max_position: int | None = None, seq_len: int | None = None):
+    """(inv_freq, factor) of ``kernels.rotary_embedding``: float64 angles per
+    position of the rotary_dim / 2 pairs, on the host, and the factor on the
+    rotated heads.
+
+    ``scaling`` is a checkpoint's ``rope_scaling`` dict.  With f_i =
+    base^(-2 i / rotary_dim), s its "factor" and o the positions the model was
+    trained on ("original_max_position_embeddings", or ``max_position``):
+
+    * "default", or None: f_i;
+    * "linear": f_i / s;
+    * "dynamic": f_i of the base b (s n / o - (s - 1))^(d / (d - 2)) for a
+      sequence of n = ``seq_len`` > o tokens, d = rotary_dim;
+    * "yarn": f_i / s where f_i turns at most beta_slow (1) times over o
+      positions, f_i where it turns at least beta_fast (32) times, with a linear
+      ramp over i between; factor 0.1 ln s + 1 unless "attention_factor" says;
+    * "llama3": f_i / s for wavelengths past o / low_freq_factor, f_i below
+      o / high_freq_factor, interpolated in o / wavelength between;
+    * "longrope": f_i / c_i with c the "long_factor" list where seq_len > o, else
+      "short_factor"; factor sqrt(1 + ln s / ln o) for s > 1, s = max_position / o
+      unless given, unless "attention_factor" says."""
+    if rotary_dim <= 0 or rotary_dim % 2:
+        raise ValueError("rotary_dim must be a positive even number")
+    i = torch.arange(rotary_dim // 2, dtype=torch.float64, device="cpu")
+    freq = float(base) ** (-2.0 * i / rotary_dim)
+    scaling = dict(scaling or {})
+    kind = scaling.get("rope_type", scaling.get("type", "default"))
+    if kind == "default":
+        return freq, 1.0
+    trained = scaling.get("original_max_position_embeddings") or max_position
+
+    def value(name):
+        if scaling.get(name) is None:
+            raise ValueError(f"rope_scaling of type {kind!r} needs {name!r}")
+        return scaling[name]
+
+    if kind != "linear" and not trained:
+        raise ValueError(f"rope_scaling of type {kind!r} needs the positions the model was trained "
+                         "on (original_max_position_embeddings or max_position)")
+    if kind == "linear":
+        return freq / float(value("factor")), 1.0
+    if kind == "dynamic":
+        s = float(value("factor"))
+        if seq_len is None or seq_len <= trained or rotary_dim <= 2:
+            return freq, 1.0
+        grown = float(base) * (s * seq_len / trained - (s - 1.0)) ** (rotary_dim / (rotary_dim - 2))
+        return grown ** (-2.0 * i / rotary_dim), 1.0
+    if kind == "yarn":
+        s = float(value("factor"))
+
+        def pair_of(turns):     # the (fractional) pair that turns so often over the trained positions
+            return rotary_dim * math.log(trained / (turns * 2 * math.pi)) / (2 * math.log(base))
+
+        low = max(math.floor(pair_of(float(scaling.get("beta_fast") or 32))), 0)
+        high = min(math.ceil(pair_of(float(scaling.get("beta_slow") or 1))), rotary_dim - 1)
+        ramp = ((i - low) / max(high - low, 0.001)).clamp(0.0, 1.0)
+        factor = scaling.get("attention_factor")
+        if factor is None:
+            factor = 0.1 * math.log(s) + 1.0 if s > 1 else 1.0
+        return freq / s * ramp + freq * (1.0 - ramp), float(factor)
+    if kind == "llama3":
+        s = float(value("factor"))
+        low, high = float(value("low_freq_factor")), float(value("high_freq_factor"))
+        turns = trained * freq / (2 * math.pi)      # trained positions over the wavelength
+        keep = ((turns - low) / (high - low)).clamp(0.0, 1.0)
+        return freq / s * (1.0 - keep) + freq * keep, 1.0
+    if kind == "longrope":
+        name = "long_factor" if seq_len is not None and seq_len > trained else "short_factor"
+        c = torch.tensor(value(name), dtype=torch.float64, device="cpu")
+        if c.shape != freq.shape:
+            raise ValueError(f"{name} must have one entry per pair")
+        factor = scaling.get("attention_factor")
+        if factor is None:
+            s = scaling.get("factor") or (max_position or trained) / trained
+            factor = math.sqrt(1.0 + math.log(s) / math.log(trained)) if s > 1 else 1.0
+        return freq / c, float(factor)
+    raise ValueError(f"unknown rope_scaling type: {kind!r}")
 
 
 class Attention(nn.Module):

@@ -44,6 +44,9 @@ enum nva_status {
 
 enum nva_kv_dtype { NVA_KV_BF16 = 0, NVA_KV_FP8_E4M3 = 1 };
 
+/* element type of entry points that take more than bf16 */
+enum nva_dtype { NVA_BF16 = 0, NVA_F16 = 1, NVA_F32 = 2 };
+
 /* Human-readable name of a status code (static string). */
 const char *nva_status_string(int status);
 
@@ -468,6 +471,91 @@ int nva_silu_mul(const void *x, int64_t x_row_stride, void *out, int64_t out_row
 int nva_linear_preferred(int32_t rows, int32_t n, int32_t k);
 int nva_linear(const void *x, int64_t x_row_stride, const void *w, void *out,
                int64_t out_row_stride, int32_t rows, int32_t n, int32_t k, void *stream);
+
+/* ---------------------------------------------------------------------
+ * Projections of few rows over 4-bit weights with group scales.  No
+ * counterpart on the reference's bf16 path; beside nva_linear.
+ * out[m, j] = bf16(sum_i x[m, i] * (code[j, i] - zero[i / group, j]) *
+ *                  scale[i / group, j] + bias[j])
+ *   in fp32: a group's sum is formed from the exact codes and then scaled, so
+ *   a weight is never rounded.  A row of x that holds an infinity or a NaN
+ *   comes out NaN; other rows are not touched by it.
+ * x: bf16 [rows, k], row stride x_row_stride; qweight: uint8 [n, k / 2]
+ *   contiguous, element 2 i in the low and 2 i + 1 in the high half of byte i;
+ *   scales: bf16 [k / group, n] contiguous; zeros: uint8 [k / group, n]
+ *   contiguous, 0..15, or NULL (8); bias: bf16 [n] or NULL.
+ * k is a multiple of group and group of 32; x, qweight and the rows of both are
+ *   16-byte aligned (x_row_stride a multiple of 8; NVA_ERR_UNSUPPORTED
+ *   otherwise).  Any number of rows: 64 at a time read the weights once.
+ * ------------------------------------------------------------------- */
+int nva_linear_w4(const void *x, int64_t x_row_stride, const void *qweight, const void *scales,
+                  const void *zeros, const void *bias, void *out, int64_t out_row_stride,
+                  int32_t rows, int32_t n, int32_t k, int32_t group, void *stream);
+
+/* ---------------------------------------------------------------------
+ * Rotary position embedding.  Covers get_rope / apply_rotary_emb
+ *   (nanovllm/layers/rotary_embedding.py:6-48) beyond the half layout over
+ *   whole heads of nva_qk_norm_rope.
+ * Pair e of a head at position p = positions[t] turns by p * inv_freq[e]:
+ *   (x, y) -> factor * (x cos - y sin, y cos + x sin), elements (e, e +
+ *   rotary_dim / 2) of the head, or (2 e, 2 e + 1) with interleaved != 0.
+ *   Elements from rotary_dim on are copied.  Angles are formed in float64, the
+ *   rotation in float32, rounded once.
+ * q [num_tokens, num_q_heads, head_dim] and k (num_k_heads 0: none) with row
+ *   and head strides and contiguous head_dim, of type dtype (nva_dtype);
+ *   inv_freq: float64 [rotary_dim / 2], device.  The outputs may be the
+ *   inputs themselves (same pointer and strides) and must not overlap them
+ *   otherwise.  head_dim <= 1024, rotary_dim even and <= 512.
+ * ------------------------------------------------------------------- */
+int nva_rotary_embedding(const int64_t *positions, const double *inv_freq, float factor,
+                         int interleaved, int dtype, const void *q, int64_t q_row_stride,
+                         int64_t q_head_stride, int32_t num_q_heads, const void *k,
+                         int64_t k_row_stride, int64_t k_head_stride, int32_t num_k_heads,
+                         int32_t num_tokens, int32_t head_dim, int32_t rotary_dim, void *q_out,
+                         int64_t q_out_row_stride, int64_t q_out_head_stride, void *k_out,
+                         int64_t k_out_row_stride, int64_t k_out_head_stride, void *stream);
+
+/* ---------------------------------------------------------------------
+ * Paged attention of a batch whose sequences share a long prefix.
+ * The result of nva_paged_attention_varlen / _decode with the same arguments,
+ *   where the first prefix_len keys of every sequence are those that row 0 of
+ *   block_tables lists (the same pages, or copies of them): the prefix's keys
+ *   are read once for the query rows of all sequences together, each
+ *   sequence's other keys by itself, and the parts are joined by their
+ *   log-sum-exp.  Row 0 must list the whole prefix, whatever sequence 0's
+ *   length.  A sequence shorter than the prefix sees its own length of it.
+ *   prefix_len >= 0; the part beyond its last multiple of 32 keys is read
+ *   through each sequence's own row.  Everything else as for K1: strides,
+ *   dtypes, scales, the clip by max_seqlen_q / max_seqlen_k (which count the
+ *   prefix), block ids outside the cache.  Rows of no sequence are not written.
+ * workspace: nva_shared_prefix_workspace_size(...) bytes, 16-byte aligned, no
+ *   initialisation; sized for the call's own shape.
+ * ------------------------------------------------------------------- */
+size_t nva_shared_prefix_workspace_size(int32_t num_seqs, int32_t num_tokens, int32_t num_q_heads,
+                                        int32_t num_kv_heads, int32_t head_dim,
+                                        int32_t max_seqlen_q, int32_t max_seqlen_k,
+                                        int32_t prefix_len);
+
+int nva_shared_prefix_attention_varlen(
+    const void *q, int64_t q_row_stride, int64_t q_head_stride, const void *k_cache,
+    const void *v_cache, int kv_dtype, int64_t cache_block_stride, int64_t cache_token_stride,
+    int64_t cache_head_stride, int32_t num_blocks, int32_t block_size,
+    const int32_t *cu_seqlens_q, const int32_t *cu_seqlens_k, const int32_t *block_tables,
+    int64_t block_table_stride, int32_t max_blocks_per_seq, int32_t num_seqs, int32_t num_tokens,
+    int32_t max_seqlen_q, int32_t max_seqlen_k, int32_t prefix_len, int32_t num_q_heads,
+    int32_t num_kv_heads, int32_t head_dim, float softmax_scale, const float *k_scale,
+    const float *v_scale, void *out, int64_t out_row_stride, int64_t out_head_stride,
+    void *workspace, size_t workspace_bytes, void *stream);
+
+int nva_shared_prefix_attention_decode(
+    const void *q, int64_t q_row_stride, int64_t q_head_stride, const void *k_cache,
+    const void *v_cache, int kv_dtype, int64_t cache_block_stride, int64_t cache_token_stride,
+    int64_t cache_head_stride, int32_t num_blocks, int32_t block_size,
+    const int32_t *cache_seqlens, const int32_t *block_tables, int64_t block_table_stride,
+    int32_t max_blocks_per_seq, int32_t num_seqs, int32_t max_seqlen_k, int32_t prefix_len,
+    int32_t num_q_heads, int32_t num_kv_heads, int32_t head_dim, float softmax_scale,
+    const float *k_scale, const float *v_scale, void *out, int64_t out_row_stride,
+    int64_t out_head_stride, void *workspace, size_t workspace_bytes, void *stream);
 
 #ifdef __cplusplus
 }
