@@ -595,9 +595,13 @@ PyObject* linear_w4(PyObject*, PyObject* const* v, Py_ssize_t n) {
       need(out.size(0) == rows && out.size(1) == m && out.stride(0) >= m);
     }
     void* s = current_stream(a.device);
+    const size_t bytes = nva_linear_w4_workspace_size(rows, m, k, group);
+    at::Tensor parts;
+    if (bytes) parts = empty_bytes(bytes, x);
     launch([&] {
       return nva_linear_w4(x.data_ptr(), x.stride(0), w.data_ptr(), sc.data_ptr(), zeros, bias,
-                           out.data_ptr(), out.stride(0), rows, m, k, group, s);
+                           out.data_ptr(), out.stride(0), rows, m, k, group,
+                           bytes ? parts.data_ptr() : nullptr, bytes, s);
     });
     return THPVariable_Wrap(out);
   });

@@ -74,7 +74,9 @@ SIGNATURES = {
     "nva_silu_mul": (_INT, [_P, _I64, _P, _I64, _I32, _I32, _P]),
     "nva_linear_preferred": (_INT, [_I32, _I32, _I32]),
     "nva_linear": (_INT, [_P, _I64, _P, _P, _I64, _I32, _I32, _I32, _P]),
-    "nva_linear_w4": (_INT, [_P, _I64, _P, _P, _P, _P, _P, _I64, _I32, _I32, _I32, _I32, _P]),
+    "nva_linear_w4_workspace_size": (_SZ, [_I32, _I32, _I32, _I32]),
+    "nva_linear_w4": (_INT, [_P, _I64, _P, _P, _P, _P, _P, _I64, _I32, _I32, _I32, _I32, _P, _SZ,
+                             _P]),
     "nva_rotary_embedding": (_INT, [_P, _P, _F32, _INT, _INT, _P, _I64, _I64, _I32, _P, _I64, _I64,
                                     _I32, _I32, _I32, _I32, _P, _I64, _I64, _P, _I64, _I64, _P]),
     "nva_shared_prefix_workspace_size": (_SZ, [_I32, _I32, _I32, _I32, _I32, _I32, _I32, _I32]),

@@ -914,9 +914,12 @@ def linear_w4(x: torch.Tensor, qweight: torch.Tensor, scales: torch.Tensor,
     if rows > 1 and out.stride(0) < n:
         raise ValueError("out rows must not overlap")
     with torch.cuda.device(x.device):
+        nbytes = int(lib.nva_linear_w4_workspace_size(rows, n, k, group))
+        ws = torch.empty(nbytes, dtype=torch.uint8, device=x.device) if nbytes else None
         check(lib.nva_linear_w4(x.data_ptr(), x.stride(0) if rows > 1 else k, qweight.data_ptr(),
                                 scales.data_ptr(), _ptr(zeros), _ptr(bias), out.data_ptr(),
-                                out.stride(0), rows, n, k, group, _stream()), "linear_w4")
+                                out.stride(0), rows, n, k, group, _ptr(ws), nbytes, _stream()),
+              "linear_w4")
     return out
 
 

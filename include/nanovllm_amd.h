@@ -487,10 +487,15 @@ int nva_linear(const void *x, int64_t x_row_stride, const void *w, void *out,
  * k is a multiple of group and group of 32; x, qweight and the rows of both are
  *   16-byte aligned (x_row_stride a multiple of 8; NVA_ERR_UNSUPPORTED
  *   otherwise).  Any number of rows: 64 at a time read the weights once.
+ * workspace: nva_linear_w4_workspace_size(rows, n, k, group) bytes (0: none),
+ *   16-byte aligned, no initialisation: the parts of ranges of k.
  * ------------------------------------------------------------------- */
+size_t nva_linear_w4_workspace_size(int32_t rows, int32_t n, int32_t k, int32_t group);
+
 int nva_linear_w4(const void *x, int64_t x_row_stride, const void *qweight, const void *scales,
                   const void *zeros, const void *bias, void *out, int64_t out_row_stride,
-                  int32_t rows, int32_t n, int32_t k, int32_t group, void *stream);
+                  int32_t rows, int32_t n, int32_t k, int32_t group, void *workspace,
+                  size_t workspace_bytes, void *stream);
 
 /* ---------------------------------------------------------------------
  * Rotary position embedding.  Covers get_rope / apply_rotary_emb

@@ -136,14 +136,14 @@ def test_the_library_refuses_bad_products_on_the_host():
 
     def call(x=P, stride=128, w=P, s=P, z=None, b=None, out=P, out_stride=8, rows=2, n=8, k=128,
              group=32):
-        return lib.nva_linear_w4(x, stride, w, s, z, b, out, out_stride, rows, n, k, group, None)
+        return lib.nva_linear_w4(x, stride, w, s, z, b, out, out_stride, rows, n, k, group, None, 0,
+                                 None)
 
     assert call(rows=0) == _native.NVA_OK
     for kw in (dict(rows=-1), dict(n=0), dict(k=0), dict(group=0), dict(group=48), dict(x=None),
                dict(w=None), dict(s=None), dict(out=None), dict(stride=120), dict(out_stride=7)):
         assert call(**kw) == _native.NVA_ERR_ARG, kw
-    for kw in (dict(group=16), dict(stride=132), dict(x=P + 8), dict(w=P + 4), dict(s=P + 2),
-               dict(z=P + 1)):
+    for kw in (dict(group=16), dict(stride=132), dict(x=P + 8), dict(w=P + 4)):
         assert call(**kw) == _native.NVA_ERR_UNSUPPORTED, kw
 
 
