@@ -56,11 +56,11 @@ DEFAULT_GEMM_TUNING = os.path.join(ROOT, "extend-nano-vllm_amd", "nanovllm_amd",
 PMC_TRAFFIC_BYTES = int((155977.1 * 2.0 + 3072.5 * 1.0) * 1024)
 PMC_WORKLOAD = dict(preset="qwen3-8b", batch=64, k=5, prompt_min=256, prompt_max=2048,
                     max_tokens=256, seed=2, kv_layout="head_major")
-# the kernel source the counters were read on (sha256 of csrc/paged_attention.hip
-# then csrc/common.h, first 16 hex digits): the constant is quoted only while
+# the kernel source the counters were read on (sha256 of csrc/paged_attention.hip,
+# csrc/attention_tiles.h, then csrc/common.h, first 16 hex digits): the constant is quoted only while
 # the source is unchanged, since a change of the kernel's loads changes it
-PMC_ATTENTION_SOURCE = "712cac485c01457c"
-ATTENTION_SOURCES = ("paged_attention.hip", "common.h")
+PMC_ATTENTION_SOURCE = "1073c86867ef3c64"
+ATTENTION_SOURCES = ("paged_attention.hip", "attention_tiles.h", "common.h")
 
 
 def attention_source_hash() -> str:
