@@ -59,7 +59,7 @@ PMC_WORKLOAD = dict(preset="qwen3-8b", batch=64, k=5, prompt_min=256, prompt_max
 # the kernel source the counters were read on (sha256 of csrc/paged_attention.hip,
 # csrc/attention_tiles.h, then csrc/common.h, first 16 hex digits): the constant is quoted only while
 # the source is unchanged, since a change of the kernel's loads changes it
-PMC_ATTENTION_SOURCE = "1073c86867ef3c64"
+PMC_ATTENTION_SOURCE = "f2de7e1db2b334b5"
 ATTENTION_SOURCES = ("paged_attention.hip", "attention_tiles.h", "common.h")
 
 

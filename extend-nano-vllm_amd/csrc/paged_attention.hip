@@ -196,14 +196,7 @@ paged_attention_kernel(AttnParams p) {
 template <int WPT, int D>
 __global__ void __launch_bounds__(kWave * WPT, 2)
 paged_attention_tile_kernel(AttnParams p) {
-  constexpr int NTW = 4 / WPT;
-  constexpr int kThreads = kWave * WPT;
-  constexpr int kRowGran = kD * 2 / 16;                  // 16-byte granules per K or V row
-  constexpr int kHalf = kChunk * kRowGran / kThreads;    // per thread per chunk, of K (and of V)
-  constexpr int kTileVPitch = 72;                        // dwords per staged V row (transpose loads)
-  constexpr int kSlot = kChunk * (kVPitch + kTileVPitch); // dwords: K rows, then V rows
-  static_assert(WPT == 2 || WPT == 4, "two or four waves per 64-row tile");
-  __shared__ __attribute__((aligned(16))) uint32_t slots[2 * kSlot];
+  __shared__ __attribute__((aligned(16))) uint32_t slots[2 * kTileSlot];
 
   const int kvh = blockIdx.x;
   const int seq = blockIdx.y;
@@ -233,244 +226,8 @@ paged_attention_tile_kernel(AttnParams p) {
   if (note) note_rows(p, seq, qt, nsplit);
   const int kv_end = kv_begin + p.split_len < kv_limit ? kv_begin + p.split_len : kv_limit;
 
-  const int tid = threadIdx.x;
-  const int lane = tid & (kWave - 1);
-  const int wv = __builtin_amdgcn_readfirstlane(tid / kWave);
-  const int g = lane >> 4;
-  const int m16 = lane & 15;
-  const int rows = jn * p.group;
-  const float sl2 = p.scale_log2;
-
-  // ---- this wave's query operands (padding columns zero) and causal limits
-  int lim[NTW];
-  bf16x8_t qv[NTW][4];
-#pragma unroll
-  for (int nt = 0; nt < NTW; ++nt) {
-    const int n = (wv * NTW + nt) * 16 + m16;
-    const int nn = n < rows ? n : 0;
-    const int j = j0 + nn / p.group, hh = nn % p.group;
-    const uint16_t* qp = p.q + static_cast<int64_t>(q_start + j) * p.q_row_stride +
-                         static_cast<int64_t>(kvh * p.group + hh) * p.q_head_stride;
-#pragma unroll
-    for (int s = 0; s < 4; ++s) qv[nt][s] = *reinterpret_cast<const bf16x8_t*>(qp + 32 * s + 8 * g);
-    const int c = L - q_len + j;
-    lim[nt] = n < rows ? (c < L - 1 ? c : L - 1) : -1;
-  }
-
-  const int nchunks = (kv_end - kv_begin + kChunk - 1) / kChunk;
-  const int first_blk = kv_begin / p.block_size;
-  const uint32_t tokb = static_cast<uint32_t>(p.tok_stride * 2);
-  // granule i of this thread: row (tid + i * kThreads) / 16, column % 16
-  uint32_t goff[kHalf], loff[kHalf], vloff[kHalf];
-#pragma unroll
-  for (int i = 0; i < kHalf; ++i) {
-    const int gi = tid + i * kThreads;
-    goff[i] = static_cast<uint32_t>(gi / kRowGran) * tokb + (gi % kRowGran) * 16;
-    loff[i] = static_cast<uint32_t>(gi / kRowGran) * kVPitch + (gi % kRowGran) * 4;
-    vloff[i] = static_cast<uint32_t>(gi / kRowGran) * kTileVPitch + (gi % kRowGran) * 4;
-  }
-
-  // chunk c's block id (uniform), in range or not
-  auto chunk_block = [&](int c) {
-    const int kb = kv_begin + c * kChunk;
-    return __builtin_amdgcn_readlane(lane_blk, kb / p.block_size - first_blk);
-  };
-  auto load_chunk = [&](int c, uint4 (&r)[2 * kHalf]) {
-    const bool live = c < nchunks;
-    const int cc = live ? c : nchunks - 1;
-    const int kb = kv_begin + cc * kChunk;
-    const int raw = chunk_block(cc);
-    const bool valid = live && raw >= 0 && raw < p.num_blocks;
-    const int visible = kv_limit - kb < kChunk ? kv_limit - kb : kChunk;
-    const int nrec = valid ? visible * static_cast<int>(tokb) : 0;
-    const int64_t tile = (static_cast<int64_t>(valid ? raw : 0) * p.blk_stride +
-                          static_cast<int64_t>(kvh) * p.head_stride +
-                          static_cast<int64_t>(kb % p.block_size) * p.tok_stride) * 2;
-    const __amdgpu_buffer_rsrc_t kr = make_rsrc(p.k_cache + tile, nrec);
-    const __amdgpu_buffer_rsrc_t vr = make_rsrc(p.v_cache + tile, nrec);
-#pragma unroll
-    for (int i = 0; i < kHalf; ++i)
-      r[i] = __builtin_bit_cast(uint4, __builtin_amdgcn_raw_buffer_load_b128(kr, goff[i], 0,
-                                                                             kLoadStreamed));
-#pragma unroll
-    for (int i = 0; i < kHalf; ++i)
-      r[kHalf + i] = __builtin_bit_cast(
-          uint4, __builtin_amdgcn_raw_buffer_load_b128(vr, goff[i], 0, kLoadStreamed));
-  };
-  auto stage = [&](const uint4 (&r)[2 * kHalf], int slot) {
-    uint32_t* kst = slots + slot * kSlot;
-#pragma unroll
-    for (int i = 0; i < kHalf; ++i) *reinterpret_cast<uint4*>(kst + loff[i]) = r[i];
-#pragma unroll
-    for (int i = 0; i < kHalf; ++i)
-      *reinterpret_cast<uint4*>(kst + kChunk * kVPitch + vloff[i]) = r[kHalf + i];
-  };
-
-  float m_run[NTW], l_run[NTW];
-  f32x4_t acc[NTW][8];
-#pragma unroll
-  for (int nt = 0; nt < NTW; ++nt) {
-    m_run[nt] = -INFINITY;
-    l_run[nt] = 0.0f;
-#pragma unroll
-    for (int t = 0; t < 8; ++t) acc[nt][t] = f32x4_t{0.f, 0.f, 0.f, 0.f};
-  }
-
-  auto compute = [&](int c, int slot) {
-    const int raw = chunk_block(c);
-    if (raw < 0 || raw >= p.num_blocks) return;       // invalid block: its keys are masked
-    const int kb = kv_begin + c * kChunk;
-    const uint32_t* kst = slots + slot * kSlot;
-    const uint32_t* vst = kst + kChunk * kVPitch;
-    f32x4_t sacc[2][NTW];
-#pragma unroll
-    for (int kt = 0; kt < 2; ++kt)
-#pragma unroll
-      for (int nt = 0; nt < NTW; ++nt) sacc[kt][nt] = f32x4_t{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-    for (int s = 0; s < 4; ++s) {
-      bf16x8_t kop[2];
-#pragma unroll
-      for (int kt = 0; kt < 2; ++kt)
-        kop[kt] = *reinterpret_cast<const bf16x8_t*>(kst + (16 * kt + m16) * kVPitch + 16 * s + 4 * g);
-#pragma unroll
-      for (int nt = 0; nt < NTW; ++nt)
-#pragma unroll
-        for (int kt = 0; kt < 2; ++kt) sacc[kt][nt] = mfma(kop[kt], qv[nt][s], sacc[kt][nt]);
-    }
-    // masked only past a causal limit, behind a uniform branch (as above)
-    const bool full = kb + kChunk - 1 <= L - q_len + j0 && kb + kChunk <= kv_limit;
-    if (!full) {
-      const int rel = kb + 4 * g;
-#pragma unroll
-      for (int nt = 0; nt < NTW; ++nt)
-#pragma unroll
-        for (int kt = 0; kt < 2; ++kt)
-#pragma unroll
-          for (int i = 0; i < 4; ++i)
-            if (rel + kt * 16 + i > lim[nt]) sacc[kt][nt][i] = -INFINITY;
-    }
-    bf16x8_t pb[NTW];
-#pragma unroll
-    for (int nt = 0; nt < NTW; ++nt) {
-      float sv[8];
-      float cmax = -INFINITY;
-#pragma unroll
-      for (int kt = 0; kt < 2; ++kt) {
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const float v = sacc[kt][nt][i];
-          sv[kt * 4 + i] = v;
-          cmax = fmaxf(cmax, v);
-        }
-      }
-      cmax = max_xor16(cmax);
-      cmax = max_xor32(cmax);
-      cmax *= sl2;
-      const bool need = cmax > m_run[nt] + kRescaleSlack;
-      if (__any(need)) {
-        const float m_new = need ? cmax : m_run[nt];
-        const float alpha = need ? exp2f_fast(m_run[nt] - m_new) : 1.0f;
-        l_run[nt] *= alpha;
-        m_run[nt] = m_new;
-#pragma unroll
-        for (int t = 0; t < 8; ++t) {
-#pragma unroll
-          for (int i = 0; i < 4; ++i) acc[nt][t][i] *= alpha;
-        }
-      }
-      const float msub = m_run[nt] == -INFINITY ? 0.0f : m_run[nt];
-      float psum = 0.0f;
-      f32x2_t pv[4];
-#pragma unroll
-      for (int k = 0; k < 8; ++k) {
-        const float e = exp2f_fast(__builtin_fmaf(sv[k], sl2, -msub));
-        pv[k >> 1][k & 1] = e;
-        psum += e;
-      }
-      l_run[nt] += psum;
-      uint4 pk;
-      pk.x = __builtin_bit_cast(uint32_t, __builtin_convertvector(pv[0], bf16x2_t));
-      pk.y = __builtin_bit_cast(uint32_t, __builtin_convertvector(pv[1], bf16x2_t));
-      pk.z = __builtin_bit_cast(uint32_t, __builtin_convertvector(pv[2], bf16x2_t));
-      pk.w = __builtin_bit_cast(uint32_t, __builtin_convertvector(pv[3], bf16x2_t));
-      pb[nt] = __builtin_bit_cast(bf16x8_t, pk);
-    }
-    // O^T += V^T . P^T through the LDS transpose load (v_operand_tr): tile
-    // (pp, hf) covers d = 32 pp + 8 (m / 4) + 4 hf + m % 4.  Against four
-    // 4-byte reads and eight byte permutes per tile pair (the one-wave
-    // segments' form), this removes 32 of the chunk's ~87 VALU instructions
-    // per wave: config 5 417 -> 407 us per call, output bits unchanged.
-#pragma unroll
-    for (int pp = 0; pp < 4; ++pp) {
-#pragma unroll
-      for (int hf = 0; hf < 2; ++hf) {
-        const bf16x8_t va = v_operand_tr(vst, kTileVPitch, lane, pp, hf);
-#pragma unroll
-        for (int nt = 0; nt < NTW; ++nt) acc[nt][2 * pp + hf] = mfma(va, pb[nt], acc[nt][2 * pp + hf]);
-      }
-    }
-  };
-
-  // ---- D chunks in flight in registers, two LDS slots: step c computes
-  // chunk c from slot c & 1, stages chunk c + 1 (loaded D steps ago) into
-  // the other slot, refills its registers with chunk c + 1 + D, and one
-  // barrier publishes the staged chunk and frees slot c & 1.
-  uint4 buf[D][2 * kHalf];
-#pragma unroll
-  for (int d = 0; d < D; ++d) load_chunk(d, buf[d]);
-  stage(buf[0], 0);
-  load_chunk(D, buf[0]);
-  __syncthreads();
-  for (int cb = 0; cb < nchunks; cb += D) {
-#pragma unroll
-    for (int d = 0; d < D; ++d) {
-      const int c = cb + d;
-      if (c < nchunks) compute(c, c & 1);
-      const int nb = (d + 1) % D;          // a constant once the loop is unrolled
-      stage(buf[nb], (c + 1) & 1);
-      load_chunk(c + 1 + D, buf[nb]);
-      __syncthreads();
-    }
-  }
-
-  // ---- finish: this wave's columns, straight from registers (lane (g, m16)
-  // holds d = 32 pp + 8 g + 0..7 of query column m16: d .. d + 3 in tile
-  // 2 pp, d + 4 .. d + 7 in tile 2 pp + 1)
-#pragma unroll
-  for (int nt = 0; nt < NTW; ++nt) {
-    float lsum = l_run[nt];
-    lsum = sum_xor16(lsum);
-    lsum = sum_xor32(lsum);
-    const float inv = lsum > 0.0f ? 1.0f / lsum : 0.0f;
-    const int n = (wv * NTW + nt) * 16 + m16;
-    if (n < rows) {
-      const int j = j0 + n / p.group, hh = n % p.group;
-      const int tok = q_start + j;
-      const int h = kvh * p.group + hh;
-      const int64_t slot = (static_cast<int64_t>(tok) * p.hq + h) * p.max_splits + split;
-#pragma unroll
-      for (int pp = 0; pp < 4; ++pp) {
-        float o[8];
-#pragma unroll
-        for (int e = 0; e < 2; ++e)
-#pragma unroll
-          for (int i = 0; i < 4; ++i) o[4 * e + i] = acc[nt][2 * pp + e][i] * inv;
-        const int d0 = 32 * pp + 8 * g;
-        if (nsplit == 1) {
-          uint16_t* op = p.out + static_cast<int64_t>(tok) * p.out_row_stride +
-                         static_cast<int64_t>(h) * p.out_head_stride + d0;
-          *reinterpret_cast<uint4*>(op) = make_uint4(pack_bf16(o[0], o[1]), pack_bf16(o[2], o[3]),
-                                                     pack_bf16(o[4], o[5]), pack_bf16(o[6], o[7]));
-        } else {
-          float* wo = p.ws_o + slot * kD + d0;
-          *reinterpret_cast<float4*>(wo) = make_float4(o[0], o[1], o[2], o[3]);
-          *reinterpret_cast<float4*>(wo + 4) = make_float4(o[4], o[5], o[6], o[7]);
-        }
-      }
-      if (nsplit > 1 && g == 0) p.ws_lse[slot] = lsum > 0.0f ? m_run[nt] + __log2f(lsum) : -INFINITY;
-    }
-  }
+  attend_tile<WPT, D>(p, slots, kvh, q_start, q_len, L, j0, jn, kv_limit, kv_begin, kv_end, split, nsplit,
+                      lane_blk);
   if (clip_owner) clear_clipped_rows(p, q_start, q_len, q_raw, threadIdx.x, blockDim.x);
 }
 

@@ -1,5 +1,4 @@
-// Paged attention of a batch whose sequences share a long prefix (gfx950,
-// MFMA 32x32x16 bf16).
+// Paged attention of a batch whose sequences share a long prefix (gfx950).
 //
 // The softmax over a row's keys is joined from parts: for a part P of the keys
 //   m_P = max s, l_P = sum exp(s - m_P), o_P = sum exp(s - m_P) v / l_P,
@@ -8,219 +7,74 @@
 // computed for tiles of query rows of all sequences together: each K and V byte
 // of the prefix is read once per tile instead of once per sequence, and the
 // products run on full matrix tiles.  Each sequence's own keys are parts of
-// tiles of its own rows.
+// tiles of its own rows.  Parts, sums and states are fp32; a probability is
+// rounded to bf16 for the product with V (relative 2^-8, as in the paged
+// attention), the output once more.
 //
-// Two launches: the parts (prefix and own keys side by side in one grid, so that
-// the matrix work of the one runs beside the memory stream of the other), then
-// the join.
+// Two launches: the parts, then the join.  The parts of the prefix and of the own
+// keys are units of one grid, two workgroups a CU, prefix units first: they
+// are the longer ones, bound by the matrix cores, and the own keys' units, bound
+// by the memory, run in the places beside and behind them.
 //
-// A unit of work is a tile of up to 32 NW query rows (NW waves of 32 columns)
-// of one kv head against a range of keys, 64 keys a step:
-//   * S^T = K . Q^T with keys as M: lane 32 h + c holds, for query column c, the
-//     keys 8 b + 4 h + i (b, i = 0..3) of each 32-key tile in accumulator
-//     element 4 b + i.  Elements 8 t .. 8 t + 7 are the k-slots of lane half h
-//     in the B operand of slice t of O^T += V^T . P^T, if slot j of half h stands
-//     for key 16 t + 8 (j / 4) + 4 h + j % 4, so P goes from accumulator to
-//     operand by rounding to bf16 alone (relative 2^-9 per probability, as the
-//     paged attention does), and V^T is read from LDS in that key order by two
-//     transpose loads.  Sums and states are fp32.
-//   * K/V tiles go through registers two steps ahead and one of two LDS buffers
-//     one step ahead, one barrier a step.  FP8 pages become bf16 on the way.
-#include "common.h"
+//   * Prefix units and sequences of more than 32 rows: wide_unit below.
+//   * Own keys of up to 32 rows: attend_segment, four waves sharing a part, each
+//     streaming chunks of its own without a barrier.
+#include <math.h>
+
+#include "attention_tiles.h"
 
 namespace nva {
 namespace {
 
-constexpr int kD = 128;
-constexpr int kKeys = 64;                            // keys of a step
-constexpr int kKPitch = 68, kVPitch = 80;            // dwords per staged row
-constexpr int kBuf = kKeys * (kKPitch + kVPitch);
-constexpr float kLog2e = 1.4426950408889634f;
-constexpr float kRescaleSlack = 8.0f;                // log2 headroom before the running max moves
-
-typedef __attribute__((ext_vector_type(2))) __bf16 bf16x2_t;
-typedef __attribute__((ext_vector_type(2))) float f32x2_t;
-typedef __attribute__((ext_vector_type(16))) float f32x16_t;
-typedef __attribute__((ext_vector_type(4))) short s16x4_t;
-typedef __attribute__((address_space(3))) s16x4_t lds_s16x4_t;
+constexpr int kWaves = 4;
+constexpr int kThreads = kWave * kWaves;
+constexpr int kTileRows = 32 * kWaves;               // query rows of a wide tile
+constexpr int kParkPitch = kD + 4;                   // floats per row of a part on its way out
+constexpr int kSegDwords = 2 * kWaves * kVStage;     // attend_segment's stages, then its query operands
+constexpr int kWideDwords = 2 * kWideBuf;
+static_assert(kTileRows * kParkPitch <= kWideDwords, "a tile's part fits the buffers");
 
 struct PrefixParams {
-  const uint16_t* q;
-  int64_t q_row_stride, q_head_stride;
-  const uint8_t* k_cache;
-  const uint8_t* v_cache;
-  int64_t blk_stride, tok_stride, head_stride;       // elements
-  int32_t num_blocks, block_size;
-  const int32_t* cu_q;                               // null: row i is sequence i
-  const int32_t* cu_k;                               // non-null: L_i = cu_k[i+1] - cu_k[i]
-  const int32_t* seqlens;                            // otherwise L_i = seqlens[i]
-  const int32_t* block_tables;
-  int64_t bt_stride;
-  int32_t bt_cols;
-  int32_t num_seqs, num_tokens, max_q, max_k;
-  int32_t hq, hkv, group;
-  float scale_log2;
-  const float* k_scale;
-  const float* v_scale;
-  uint16_t* out;
-  int64_t out_row_stride, out_head_stride;
-  float* ws_o;                                       // [token][head][part][kD], normalised
-  float* ws_lse;                                     // [token][head][part], log2
-  int32_t* row_parts;                                // [token] parts of its own keys, -1: no output but zeros
-  // the plan
+  AttnParams a;        // max_splits: the parts of a row; row_nsplit: its own keys' (-1: none, zeros)
   int32_t prefix;                                    // shared keys (a multiple of 32)
   int32_t prefix_split, prefix_parts;                // keys of a prefix part, parts
   int32_t own_split, own_parts;                      // the same of a sequence's own keys (parts: bound)
-  int32_t qtile, prefix_tiles, own_tiles;            // query positions of a tile, tiles
+  int32_t prefix_tiles, own_tiles;                   // tiles of a.qtile query positions
   int32_t prefix_units, own_units;                   // per kv head
 };
 
-__device__ __forceinline__ float exp2f_fast(float x) { return __builtin_amdgcn_exp2f(x); }
-
-// over the lane pair (l, l ^ 32), by the swap of the two halves; the results are
-// read into integers first (a bit cast of the second element of the builtin's
-// result vector compiles to the first, ROCm 7.2)
-__device__ __forceinline__ float max_halves(float x) {
-  const uint32_t u = __builtin_bit_cast(uint32_t, x);
-  const auto r = __builtin_amdgcn_permlane32_swap(u, u, false, false);
-  const uint32_t lo = r[0], hi = r[1];
-  return fmaxf(__builtin_bit_cast(float, lo), __builtin_bit_cast(float, hi));
-}
-__device__ __forceinline__ float sum_halves(float x) {
-  const uint32_t u = __builtin_bit_cast(uint32_t, x);
-  const auto r = __builtin_amdgcn_permlane32_swap(u, u, false, false);
-  const uint32_t lo = r[0], hi = r[1];
-  return __builtin_bit_cast(float, lo) + __builtin_bit_cast(float, hi);
-}
-
-__device__ __forceinline__ f32x16_t mfma32(bf16x8_t a, bf16x8_t b, f32x16_t c) {
-  return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0);
-}
-
-// 8 e4m3 bytes as bf16, exact
-__device__ __forceinline__ bf16x8_t fp8x8_to_bf16(uint2 w) {
-  const bf16x2_t a = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w.x, 1.0f, false);
-  const bf16x2_t b = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w.x, 1.0f, true);
-  const bf16x2_t c = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w.y, 1.0f, false);
-  const bf16x2_t d = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w.y, 1.0f, true);
-  return __builtin_bit_cast(bf16x8_t,
-                            make_uint4(__builtin_bit_cast(uint32_t, a), __builtin_bit_cast(uint32_t, b),
-                                       __builtin_bit_cast(uint32_t, c), __builtin_bit_cast(uint32_t, d)));
-}
-
-// V^T operand of head_dim tile dt (d = 32 dt + lane % 32) and key slice t (16
-// keys): transpose load r (0, 1) hands lane 32 h + c the keys 16 t + 8 r + 4 h ..
-// + 3.  ds_read_b64_tr_b16 gives lane l element e of the 8-byte piece that lane
-// 16 (l / 16) + 4 e + (l % 16) / 4 addressed, at position (l % 16) % 4.
-__device__ __forceinline__ bf16x8_t v_operand(const uint32_t* rows, int lane, int t, int dt) {
-  const int h = lane >> 5, dh = (lane >> 4) & 1, i = lane & 15;
-  uint32_t* p0 = const_cast<uint32_t*>(rows) + (16 * t + 4 * h + (i >> 2)) * kVPitch + 16 * dt + 8 * dh +
-                 2 * (i & 3);
-  const s16x4_t lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4_t*)(p0));
-  const s16x4_t hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4_t*)(p0 + 8 * kVPitch));
-  return bf16x8_t{lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
-}
-
-// Query rows and keys of a sequence.  A sequence clipped to its first max_q
-// rows also drops the keys of the rows cut, so that each kept row j still sees
-// keys [0, L - raw + j]; then at most max_k keys are seen.
-struct Geometry {
-  int q_start, q_len, raw, L;
-};
-__device__ __forceinline__ Geometry geometry(const PrefixParams& p, int seq) {
-  int q0 = seq, q1 = seq + 1, k0 = 0;
-  const int k1 = (p.cu_k ? p.cu_k + 1 : p.seqlens)[seq];
-  if (p.cu_q) {
-    q0 = p.cu_q[seq];
-    q1 = p.cu_q[seq + 1];
-  }
-  if (p.cu_k) k0 = p.cu_k[seq];
-  Geometry r;
-  r.q_start = q0;
-  r.raw = q1 - q0;
-  if (q0 < 0 || q0 >= p.num_tokens) r.raw = 0;
-  else if (r.raw > p.num_tokens - q0) r.raw = p.num_tokens - q0;
-  if (r.raw < 0) r.raw = 0;
-  r.q_len = r.raw > p.max_q ? p.max_q : r.raw;
-  r.L = k1 - k0 - (r.raw - r.q_len);
-  r.L = r.L > p.max_k ? p.max_k : r.L;
-  return r;
-}
-
-// the id of the block that lane i's column is from `first` on, -1 past the table
-__device__ __forceinline__ int block_ids(const PrefixParams& p, const int32_t* table, int key) {
-  const int col = key / p.block_size + static_cast<int>(threadIdx.x & (kWave - 1));
-  return col < p.bt_cols ? table[col] : -1;
-}
-
-template <int NW, bool FP8>
-__global__ void __launch_bounds__(kWave * NW, 2) shared_prefix_kernel(PrefixParams p) {
-  constexpr int kThreads = kWave * NW;
+// A tile of query rows of one kv head (positions tok0 .. tok0 + jn - 1 of the
+// batch, all heads of the group) against the keys [kv_begin, kv_end) of a block
+// table, 64 keys a step; the part goes to the workspace.
+//   * A wave holds 32 rows on the 32x32x16 MFMA; HALVES (tiles of up to 64 rows):
+//     wave w has row group w % 2 and takes keys 32 (w / 2) .. + 31 of each
+//     step, and the two halves' states meet in LDS.
+//   * S^T = K . Q^T with keys as M: lane 32 h + c holds, for query column c, the
+//     keys 8 b + 4 h + i (b, i = 0..3) of a 32-key tile in accumulator element
+//     4 b + i.  Elements 8 t .. 8 t + 7 are the k-slots of lane half h in the B
+//     operand of slice t of O^T += V^T . P^T, if slot j of half h stands for key
+//     16 t + 8 (j / 4) + 4 h + j % 4, so P goes from accumulator to operand by
+//     rounding alone, and V^T is read from LDS in that order by two transpose
+//     loads (wide_v_operand).
+//   * K/V go through registers two steps ahead and one of two LDS buffers one
+//     step ahead, one barrier a step.  FP8 pages become bf16 on the way.
+//   * The part leaves through LDS as whole rows of 512 bytes.
+// last_key[j]: the last key that position tok0 + j sees (less than 0: none).
+template <bool HALVES, bool FP8>
+__device__ __forceinline__ void wide_unit(const AttnParams& p, uint32_t* lds, const int32_t* last_key,
+                                          const int kvh, const int tok0, const int jn,
+                                          const int kv_begin, const int kv_end, const int part,
+                                          const int32_t* table) {
   constexpr int kEsz = FP8 ? 1 : 2;
   constexpr int kRowGran = kD * kEsz / 16;               // 16-byte granules per K or V row
-  constexpr int kPer = kKeys * kRowGran / kThreads;      // a thread's granules of K (and of V)
+  constexpr int kPer = kWideKeys * kRowGran / kThreads;  // a thread's granules of K (and of V)
+  constexpr int kTiles = HALVES ? 1 : 2;                 // 32-key tiles of a wave's step
   static_assert(kPer >= 1, "every thread loads at least one granule");
-  __shared__ __attribute__((aligned(16))) uint32_t lds[2 * kBuf];
-  __shared__ int32_t last_key[32 * NW];                  // of each query position of the tile, -1: none
-
-  const int kvh = blockIdx.x % p.hkv;
-  // prefix units are spread evenly among the others
-  const int all = p.prefix_units + p.own_units;
-  const int u = blockIdx.x / p.hkv;
-  const int before = static_cast<int>(static_cast<int64_t>(u) * p.prefix_units / all);
-  const bool is_prefix = static_cast<int>(static_cast<int64_t>(u + 1) * p.prefix_units / all) > before;
-
-  int tok0, jn, kv_begin, kv_end, part;
-  const int32_t* table;
-  if (is_prefix) {
-    const int tile = before % p.prefix_tiles, split = before / p.prefix_tiles;
-    tok0 = tile * p.qtile;
-    jn = p.num_tokens - tok0 < p.qtile ? p.num_tokens - tok0 : p.qtile;
-    kv_begin = split * p.prefix_split;
-    kv_end = kv_begin + p.prefix_split < p.prefix ? kv_begin + p.prefix_split : p.prefix;
-    part = split;
-    table = p.block_tables;
-    // every position's last visible key, from the sequence that holds it
-    for (int i = threadIdx.x; i < jn; i += kThreads) last_key[i] = -1;
-    __syncthreads();
-    for (int seq = p.cu_q ? static_cast<int>(threadIdx.x) : tok0 + static_cast<int>(threadIdx.x);
-         seq < (p.cu_q ? p.num_seqs : tok0 + jn); seq += kThreads) {
-      const Geometry g = geometry(p, seq);
-      const int lo = g.q_start > tok0 ? g.q_start : tok0;
-      const int hi = g.q_start + g.q_len < tok0 + jn ? g.q_start + g.q_len : tok0 + jn;
-      for (int t = lo; t < hi; ++t) last_key[t - tok0] = g.L - g.q_len + (t - g.q_start);
-    }
-    __syncthreads();
-  } else {
-    int rest = u - before;
-    const int seq = rest % p.num_seqs;
-    rest /= p.num_seqs;
-    const int qt = p.own_tiles - 1 - rest % p.own_tiles, split = rest / p.own_tiles;
-    Geometry g = geometry(p, seq);
-    const int j0 = qt * p.qtile;
-    jn = g.q_len - j0 < p.qtile ? g.q_len - j0 : p.qtile;
-    jn = __builtin_amdgcn_readfirstlane(jn);
-    const int limit = __builtin_amdgcn_readfirstlane(g.L - g.q_len + j0 + jn);   // keys seen by the last row
-    tok0 = __builtin_amdgcn_readfirstlane(g.q_start + j0);
-    kv_begin = p.prefix + split * p.own_split;
-    kv_end = kv_begin + p.own_split < limit ? kv_begin + p.own_split : limit;
-    part = p.prefix_parts + split;
-    table = p.block_tables + static_cast<int64_t>(seq) * p.bt_stride;
-    if (kvh == 0 && split == 0) {
-      // what the join reads of each row: the parts written for it
-      const int parts = limit > p.prefix ? (limit - p.prefix + p.own_split - 1) / p.own_split : 0;
-      for (int j = threadIdx.x; j < jn; j += kThreads) p.row_parts[tok0 + j] = parts;
-      if (qt == 0)
-        for (int j = g.q_len + threadIdx.x; j < g.raw; j += kThreads) p.row_parts[g.q_start + j] = -1;
-    }
-    if (jn <= 0 || kv_begin >= kv_end) return;
-    for (int j = threadIdx.x; j < jn; j += kThreads) last_key[j] = g.L - g.q_len + j0 + j;
-    __syncthreads();
-  }
-
   const int tid = threadIdx.x;
   const int lane = tid & (kWave - 1);
   const int wv = __builtin_amdgcn_readfirstlane(tid / kWave);
+  const int rw = HALVES ? wv & 1 : wv;                   // row group
+  const int half = HALVES ? wv >> 1 : 0;
   const int h = lane >> 5;
   const int col = lane & 31;
   const int rows = jn * p.group;
@@ -233,13 +87,13 @@ __global__ void __launch_bounds__(kWave * NW, 2) shared_prefix_kernel(PrefixPara
 
   // ---- this lane's query column (a padding column repeats row 0 and is not
   // stored), its last visible key, and the wave's least and greatest
-  const int n = 32 * wv + col;
+  const int n = 32 * rw + col;
   const int nn = n < rows ? n : 0;
   const int jc = nn / p.group, hc = kvh * p.group + nn % p.group;
-  const int64_t tok = tok0 + jc;
   bf16x8_t qv[8];
   {
-    const uint16_t* qp = p.q + tok * p.q_row_stride + static_cast<int64_t>(hc) * p.q_head_stride + 8 * h;
+    const uint16_t* qp = p.q + static_cast<int64_t>(tok0 + jc) * p.q_row_stride +
+                         static_cast<int64_t>(hc) * p.q_head_stride + 8 * h;
 #pragma unroll
     for (int s = 0; s < 8; ++s) qv[s] = *reinterpret_cast<const bf16x8_t*>(qp + 16 * s);
   }
@@ -253,7 +107,7 @@ __global__ void __launch_bounds__(kWave * NW, 2) shared_prefix_kernel(PrefixPara
   }
   const int wave_full = __builtin_amdgcn_readfirstlane(least) + 1;   // keys below it are seen by every row
   // keys from it on by none
-  const int wave_end = 32 * wv < rows ? __builtin_amdgcn_readfirstlane(most) + 1 : 0;
+  const int wave_end = 32 * rw < rows ? __builtin_amdgcn_readfirstlane(most) + 1 : 0;
 
   // ---- loads: thread granule i is row (tid + i kThreads) / kRowGran of the
   // step; its 32-key half is the same for the whole wave.  The halves have
@@ -269,11 +123,15 @@ __global__ void __launch_bounds__(kWave * NW, 2) shared_prefix_kernel(PrefixPara
     const int row = gi / kRowGran, c = gi % kRowGran;
     upper[i] = kStepRows <= 32 ? i * kStepRows >= 32 : __builtin_amdgcn_readfirstlane(row) >= 32;
     goff[i] = static_cast<uint32_t>(row & 31) * tokb + c * 16;
-    kdst[i] = row * kKPitch + c * (FP8 ? 8 : 4);
-    vdst[i] = kKeys * kKPitch + row * kVPitch + c * (FP8 ? 8 : 4);
+    kdst[i] = row * kWideKPitch + c * (FP8 ? 8 : 4);
+    vdst[i] = kWideKeys * kWideKPitch + row * kWideVPitch + c * (FP8 ? 8 : 4);
   }
   // lane i of lane_blk holds the id of the i-th block from the one ld_blk counts from
-  int lane_blk = block_ids(p, table, kv_begin);
+  auto block_ids = [&](int key) {
+    const int c = key / p.block_size + lane;
+    return c < p.bt_cols ? table[c] : -1;
+  };
+  int lane_blk = block_ids(kv_begin);
   int ld_key = kv_begin;                                 // first key of the next half to load,
   int ld_blk = 0;                                        // its block
   int ld_tok = kv_begin % p.block_size;                  // and its token there
@@ -281,7 +139,7 @@ __global__ void __launch_bounds__(kWave * NW, 2) shared_prefix_kernel(PrefixPara
     const bool live = ld_key < kv_end;
     if (live && ld_blk >= kWave) {
       ld_blk = 0;
-      lane_blk = block_ids(p, table, ld_key);
+      lane_blk = block_ids(ld_key);
     }
     const int raw = __builtin_amdgcn_readlane(lane_blk, ld_blk & (kWave - 1));
     const bool valid = live && raw >= 0 && raw < p.num_blocks;
@@ -318,7 +176,7 @@ __global__ void __launch_bounds__(kWave * NW, 2) shared_prefix_kernel(PrefixPara
     }
   };
   auto stage = [&](const Tile& t, int b) {
-    uint32_t* base = lds + b * kBuf;
+    uint32_t* base = lds + b * kWideBuf;
 #pragma unroll
     for (int i = 0; i < kPer; ++i) {
       if constexpr (FP8) {
@@ -340,38 +198,40 @@ __global__ void __launch_bounds__(kWave * NW, 2) shared_prefix_kernel(PrefixPara
 #pragma unroll
     for (int i = 0; i < 16; ++i) acc[dt][i] = 0.0f;
 
-  auto compute = [&](int kb, int valid, int b) {
-    if (kb >= wave_end || valid == 0) return;
-    const uint32_t* kst = lds + b * kBuf;
-    const uint32_t* vst = kst + kKeys * kKPitch;
-    f32x16_t sacc[2];
+  auto compute = [&](int key0, int ok, int b) {
+    const int kb = key0 + 32 * half;                     // the wave's first key
+    if (HALVES) ok = ok >> half & 1;
+    if (kb >= wave_end || ok == 0) return;
+    const uint32_t* kst = lds + b * kWideBuf + 32 * half * kWideKPitch;
+    const uint32_t* vst = lds + b * kWideBuf + kWideKeys * kWideKPitch + 32 * half * kWideVPitch;
+    f32x16_t sacc[kTiles];
 #pragma unroll
-    for (int kt = 0; kt < 2; ++kt)
+    for (int kt = 0; kt < kTiles; ++kt)
 #pragma unroll
       for (int i = 0; i < 16; ++i) sacc[kt][i] = 0.0f;
 #pragma unroll
     for (int s = 0; s < 8; ++s)
 #pragma unroll
-      for (int kt = 0; kt < 2; ++kt) {
+      for (int kt = 0; kt < kTiles; ++kt) {
         const bf16x8_t ko =
-            *reinterpret_cast<const bf16x8_t*>(kst + (32 * kt + col) * kKPitch + 8 * s + 4 * h);
+            *reinterpret_cast<const bf16x8_t*>(kst + (32 * kt + col) * kWideKPitch + 8 * s + 4 * h);
         sacc[kt] = mfma32(ko, qv[s], sacc[kt]);
       }
-    if (kb + kKeys > wave_full || valid != 3) {
+    if (kb + 32 * kTiles > wave_full || ok != (1 << kTiles) - 1) {
 #pragma unroll
-      for (int kt = 0; kt < 2; ++kt)
+      for (int kt = 0; kt < kTiles; ++kt)
 #pragma unroll
         for (int i = 0; i < 16; ++i) {
           const int key = kb + 32 * kt + 8 * (i >> 2) + 4 * h + (i & 3);
-          if (key > lim || !((valid >> kt) & 1)) sacc[kt][i] = -INFINITY;
+          if (key > lim || !((ok >> kt) & 1)) sacc[kt][i] = -INFINITY;
         }
     }
     float cmax = sacc[0][0];
 #pragma unroll
-    for (int kt = 0; kt < 2; ++kt)
+    for (int kt = 0; kt < kTiles; ++kt)
 #pragma unroll
       for (int i = 0; i < 16; ++i) cmax = fmaxf(cmax, sacc[kt][i]);
-    cmax = max_halves(cmax) * sl2;
+    cmax = max_xor32(cmax) * sl2;
     const bool need = cmax > m_run + kRescaleSlack;
     if (__any(need)) {
       const float m_new = need ? cmax : m_run;
@@ -384,10 +244,10 @@ __global__ void __launch_bounds__(kWave * NW, 2) shared_prefix_kernel(PrefixPara
         for (int i = 0; i < 16; ++i) acc[dt][i] *= alpha;
     }
     const float msub = m_run == -INFINITY ? 0.0f : m_run;
-    bf16x8_t pb[4];
+    bf16x8_t pb[2 * kTiles];
     float psum[2] = {0.0f, 0.0f};
 #pragma unroll
-    for (int t = 0; t < 4; ++t) {
+    for (int t = 0; t < 2 * kTiles; ++t) {
       uint32_t w[4];
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
@@ -403,15 +263,15 @@ __global__ void __launch_bounds__(kWave * NW, 2) shared_prefix_kernel(PrefixPara
     }
     l_run += psum[0] + psum[1];
 #pragma unroll
-    for (int t = 0; t < 4; ++t)
+    for (int t = 0; t < 2 * kTiles; ++t)
 #pragma unroll
-      for (int dt = 0; dt < 4; ++dt) acc[dt] = mfma32(v_operand(vst, lane, t, dt), pb[t], acc[dt]);
+      for (int dt = 0; dt < 4; ++dt) acc[dt] = mfma32(wide_v_operand(vst, lane, t, dt), pb[t], acc[dt]);
   };
 
   // step c computes tile c from buffer c & 1, stages tile c + 1 into the other
   // buffer and loads tile c + 2; the barrier publishes the staged tile and
   // frees the computed one
-  const int ntiles = (kv_end - kv_begin + kKeys - 1) / kKeys;
+  const int ntiles = (kv_end - kv_begin + kWideKeys - 1) / kWideKeys;
   Tile t;
   load_tile(t);
   stage(t, 0);
@@ -419,7 +279,7 @@ __global__ void __launch_bounds__(kWave * NW, 2) shared_prefix_kernel(PrefixPara
   load_tile(t);
   __syncthreads();
   for (int c = 0; c < ntiles; ++c) {
-    compute(kv_begin + c * kKeys, valid, c & 1);
+    compute(kv_begin + c * kWideKeys, valid, c & 1);
     if (c + 1 < ntiles) {
       stage(t, (c + 1) & 1);
       valid = t.valid;
@@ -428,20 +288,132 @@ __global__ void __launch_bounds__(kWave * NW, 2) shared_prefix_kernel(PrefixPara
     __syncthreads();
   }
 
-  // ---- the part: elements 4 b + i of tile dt are d = 32 dt + 8 b + 4 h + i
-  const float lsum = sum_halves(l_run);
-  const float inv = lsum > 0.0f ? vscale / lsum : 0.0f;
-  if (n < rows) {
-    const int64_t slot = (tok * p.hq + hc) * (p.prefix_parts + p.own_parts) + part;
-    float* wo = p.ws_o + slot * kD;
+  // ---- the part: elements 4 b + i of tile dt are d = 32 dt + 8 b + 4 h + i.
+  // Every buffer is free behind the loop's last barrier.
+  float* const park = reinterpret_cast<float*>(lds) + rw * 32 * kParkPitch;
+  if constexpr (HALVES) {
+    // the second half's waves park their states (behind the two row groups'
+    // parts), the first's take them in
+    float* const other = reinterpret_cast<float*>(lds) + 2 * 32 * kParkPitch + rw * kWave * 66;
+    static_assert(2 * 32 * kParkPitch + 2 * kWave * 66 <= kWideDwords, "parked states fit");
+    if (half == 1) {
+#pragma unroll
+      for (int dt = 0; dt < 4; ++dt)
+#pragma unroll
+        for (int b = 0; b < 4; ++b)
+          reinterpret_cast<f32x4_t*>(other)[(4 * dt + b) * kWave + lane] =
+              f32x4_t{acc[dt][4 * b], acc[dt][4 * b + 1], acc[dt][4 * b + 2], acc[dt][4 * b + 3]};
+      other[64 * kWave + lane] = m_run;
+      other[65 * kWave + lane] = l_run;
+    }
+    __syncthreads();
+    if (half == 1) return;
+    const float m1 = other[64 * kWave + lane], l1 = other[65 * kWave + lane];
+    const float M = fmaxf(m_run, m1);
+    const float f0 = m_run == -INFINITY ? 0.0f : exp2f_fast(m_run - M);
+    const float f1 = m1 == -INFINITY ? 0.0f : exp2f_fast(m1 - M);
+    m_run = M;
+    l_run = f0 * l_run + f1 * l1;
 #pragma unroll
     for (int dt = 0; dt < 4; ++dt)
 #pragma unroll
-      for (int b = 0; b < 4; ++b)
-        *reinterpret_cast<float4*>(wo + 32 * dt + 8 * b + 4 * h) =
-            make_float4(acc[dt][4 * b] * inv, acc[dt][4 * b + 1] * inv, acc[dt][4 * b + 2] * inv,
-                        acc[dt][4 * b + 3] * inv);
-    if (h == 0) p.ws_lse[slot] = lsum > 0.0f ? m_run + __log2f(lsum) : -INFINITY;
+      for (int b = 0; b < 4; ++b) {
+        const f32x4_t o = reinterpret_cast<const f32x4_t*>(other)[(4 * dt + b) * kWave + lane];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) acc[dt][4 * b + i] = f0 * acc[dt][4 * b + i] + f1 * o[i];
+      }
+  }
+  const float lsum = sum_xor32(l_run);
+  const float inv = lsum > 0.0f ? vscale / lsum : 0.0f;
+  // through the wave's own rows of LDS, then out row by row
+#pragma unroll
+  for (int dt = 0; dt < 4; ++dt)
+#pragma unroll
+    for (int b = 0; b < 4; ++b)
+      *reinterpret_cast<float4*>(park + col * kParkPitch + 32 * dt + 8 * b + 4 * h) =
+          make_float4(acc[dt][4 * b] * inv, acc[dt][4 * b + 1] * inv, acc[dt][4 * b + 2] * inv,
+                      acc[dt][4 * b + 3] * inv);
+  lds_wave_sync();
+  const auto slot_of = [&](int r) {
+    return (static_cast<int64_t>(tok0 + r / p.group) * p.hq + kvh * p.group + r % p.group) * p.max_splits + part;
+  };
+#pragma unroll 4
+  for (int i = 0; i < 16; ++i) {
+    const int r = 32 * rw + 2 * i + h;
+    const float4 o = *reinterpret_cast<const float4*>(park + (2 * i + h) * kParkPitch + 4 * col);
+    if (r < rows) *reinterpret_cast<float4*>(p.ws_o + slot_of(r) * kD + 4 * col) = o;
+  }
+  if (n < rows && h == 0) p.ws_lse[slot_of(n)] = lsum > 0.0f ? m_run + __log2f(lsum) : -INFINITY;
+}
+
+// OWN: how the own keys' units run: tiles of 16 (1) or 32 (2) rows on
+// attend_segment, of 64 (3) on attend_tile (bf16) or wide_unit, of 128 (4) on
+// wide_unit.  FEW: prefix tiles of up to 64 rows.
+template <int OWN, bool FEW, bool FP8>
+__global__ void __launch_bounds__(kThreads, 2) shared_prefix_kernel(PrefixParams pp) {
+  constexpr int kDwords = OWN > 2 ? kWideDwords
+                          : kSegDwords + OWN * 4 * kWave * 4 > kWideDwords ? kSegDwords + OWN * 4 * kWave * 4
+                                                                           : kWideDwords;
+  __shared__ __attribute__((aligned(16))) uint32_t lds[kDwords];
+  __shared__ int32_t last_key[kTileRows];                // of each query position of a wide tile
+  const AttnParams& p = pp.a;
+  const int kvh = blockIdx.x % p.hkv;
+  const int u = blockIdx.x / p.hkv;
+  if (u < pp.prefix_units) {
+    const int tile = u % pp.prefix_tiles, split = u / pp.prefix_tiles;
+    const int tok0 = tile * p.qtile;
+    const int jn = p.num_tokens - tok0 < p.qtile ? p.num_tokens - tok0 : p.qtile;
+    const int kv_begin = split * pp.prefix_split;
+    const int kv_end = kv_begin + pp.prefix_split < pp.prefix ? kv_begin + pp.prefix_split : pp.prefix;
+    // every position's last visible key, from the sequence that holds it
+    for (int i = threadIdx.x; i < jn; i += kThreads) last_key[i] = -1;
+    __syncthreads();
+    for (int seq = p.cu_q ? static_cast<int>(threadIdx.x) : tok0 + static_cast<int>(threadIdx.x);
+         seq < (p.cu_q ? p.num_seqs : tok0 + jn); seq += kThreads) {
+      int q_start, q_len, L;
+      seq_geometry(p, seq, q_start, q_len, L);
+      const int lo = q_start > tok0 ? q_start : tok0;
+      const int hi = q_start + q_len < tok0 + jn ? q_start + q_len : tok0 + jn;
+      for (int t = lo; t < hi; ++t) last_key[t - tok0] = L - q_len + (t - q_start);
+    }
+    __syncthreads();
+    wide_unit<FEW, FP8>(p, lds, last_key, kvh, tok0, jn, kv_begin, kv_end, split, p.block_tables);
+    return;
+  }
+  int rest = u - pp.prefix_units;
+  const int seq = rest % p.num_seqs;
+  rest /= p.num_seqs;
+  const int qt = pp.own_tiles - 1 - rest % pp.own_tiles, split = rest / pp.own_tiles;
+  const int kv_begin = pp.prefix + split * pp.own_split;
+  int lane_blk = 0;
+  if constexpr (OWN <= 2 || !FP8) lane_blk = split_block_ids(p, seq, kv_begin);
+  int q_start, q_len, L, q_raw;
+  seq_geometry_uniform(p, seq, q_start, q_len, L, &q_raw);
+  const int j0 = qt * p.qtile;
+  const int jn = q_len - j0 < p.qtile ? q_len - j0 : p.qtile;
+  const int limit = L - q_len + j0 + jn;                 // keys seen by the tile's last row
+  const int kv_end = kv_begin + pp.own_split < limit ? kv_begin + pp.own_split : limit;
+  if (kvh == 0 && split == 0) {
+    // what the join reads of each row: the parts written for it
+    const int parts = limit > pp.prefix ? (limit - pp.prefix + pp.own_split - 1) / pp.own_split : 0;
+    for (int j = threadIdx.x; j < jn; j += kThreads) p.row_nsplit[q_start + j0 + j] = parts;
+    if (qt == 0)
+      for (int j = q_len + static_cast<int>(threadIdx.x); j < q_raw; j += kThreads) p.row_nsplit[q_start + j] = -1;
+  }
+  if (jn <= 0 || kv_begin >= kv_end) return;
+  if constexpr (OWN <= 2) {
+    // (a count of parts other than 1, which would mean an output)
+    attend_segment<OWN, FP8, false, kWaves>(p, lds, reinterpret_cast<bf16x8_t*>(lds + kSegDwords), kvh, seq,
+                                            q_start, q_len, L, kv_begin, kv_end, pp.prefix_parts + split, 2,
+                                            lane_blk);
+  } else if constexpr (OWN == 3 && !FP8) {
+    attend_tile<kWaves, 4>(p, lds, kvh, q_start, q_len, L, 0, jn, limit, kv_begin, kv_end,
+                           pp.prefix_parts + split, 2, lane_blk);
+  } else {
+    for (int j = threadIdx.x; j < jn; j += kThreads) last_key[j] = L - q_len + j0 + j;
+    __syncthreads();
+    wide_unit<OWN == 3, FP8>(p, lds, last_key, kvh, q_start + j0, jn, kv_begin, kv_end,
+                             pp.prefix_parts + split, p.block_tables + static_cast<int64_t>(seq) * p.bt_stride);
   }
 }
 
@@ -449,19 +421,20 @@ __global__ void __launch_bounds__(kWave * NW, 2) shared_prefix_kernel(PrefixPara
 // its parts, kBatch loads at a time, into a running maximum, weight and sum.
 constexpr int kJoinThreads = 256;
 constexpr int kBatch = 8;
-__global__ void __launch_bounds__(kJoinThreads) join_kernel(PrefixParams p) {
+__global__ void __launch_bounds__(kJoinThreads) join_kernel(PrefixParams pp) {
+  const AttnParams& p = pp.a;
   const int t = blockIdx.x;
   // rows of no sequence are left alone
   const int lo = p.cu_q ? p.cu_q[0] : 0;
   const int hi = p.cu_q ? p.cu_q[p.num_seqs] : p.num_seqs;
-  int own = p.row_parts[t];
+  int own = p.row_nsplit[t];
   if (t < lo || t >= hi) return;
   const int idx = blockIdx.y * kJoinThreads + threadIdx.x;
   if (idx >= p.hq * (kD / 4)) return;
   const int h = idx / (kD / 4), d4 = idx % (kD / 4);
-  own = own < p.own_parts ? own : p.own_parts;
-  const int parts = own < 0 ? 0 : p.prefix_parts + own;
-  const int64_t base = (static_cast<int64_t>(t) * p.hq + h) * (p.prefix_parts + p.own_parts);
+  own = own < pp.own_parts ? own : pp.own_parts;
+  const int parts = own < 0 ? 0 : pp.prefix_parts + own;
+  const int64_t base = (static_cast<int64_t>(t) * p.hq + h) * p.max_splits;
   float M = -INFINITY, wsum = 0.0f;
   float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
   for (int s0 = 0; s0 < parts; s0 += kBatch) {
@@ -490,12 +463,9 @@ __global__ void __launch_bounds__(kJoinThreads) join_kernel(PrefixParams p) {
     M = mb;
   }
   const float inv = wsum > 0.0f ? 1.0f / wsum : 0.0f;
-  auto pack = [&](float a, float b) {
-    return static_cast<uint32_t>(f32_to_bf16(a * inv)) | (static_cast<uint32_t>(f32_to_bf16(b * inv)) << 16);
-  };
   uint16_t* op = p.out + static_cast<int64_t>(t) * p.out_row_stride +
                  static_cast<int64_t>(h) * p.out_head_stride + 4 * d4;
-  *reinterpret_cast<uint2*>(op) = make_uint2(pack(o.x, o.y), pack(o.z, o.w));
+  *reinterpret_cast<uint2*>(op) = make_uint2(pack_bf16(o.x * inv, o.y * inv), pack_bf16(o.z * inv, o.w * inv));
 }
 
 // Compute units of the current device (cached per device; 256 when the query fails).
@@ -513,45 +483,89 @@ int32_t device_cus() {
 
 int32_t ceil_div(int64_t a, int64_t b) { return static_cast<int32_t>((a + b - 1) / b); }
 
-constexpr int kWaves = 4;
-constexpr int kMinPart = 256;          // keys a part has at least
+// Whether the prefix is one tile of up to 64 rows (the kernel's FEW).
+bool few_rows(const AttnParams& p) { return static_cast<int64_t>(p.num_tokens) * p.group <= 64; }
 
-// Tiles and parts of a call.  Unknown lengths are bounded by max_k.
-void make_plan(PrefixParams& p, int32_t prefix_len) {
-  p.prefix = prefix_len < p.max_k ? prefix_len / 32 * 32 : p.max_k / 32 * 32;
-  p.qtile = 32 * kWaves / p.group;
-  p.prefix_tiles = ceil_div(p.num_tokens, p.qtile);
-  p.own_tiles = ceil_div(p.max_q, p.qtile);
-  const int64_t places = 2 * static_cast<int64_t>(device_cus());
-  // prefix: parts enough to give every place of the device a unit
-  int32_t parts = static_cast<int32_t>(places / (static_cast<int64_t>(p.prefix_tiles) * p.hkv));
-  const int32_t most = p.prefix / kMinPart;
-  parts = parts < 1 ? 1 : parts;
-  parts = parts > most ? (most < 1 ? 1 : most) : parts;
-  p.prefix_split = ceil_div(ceil_div(p.prefix, parts), kKeys) * kKeys;
-  p.prefix_parts = p.prefix > 0 ? ceil_div(p.prefix, p.prefix_split) : 0;
+// How the own keys of tiles of so many rows run (the kernel's OWN).
+int own_kind(int64_t rows) { return rows <= 16 ? 1 : rows <= 32 ? 2 : rows <= 64 ? 3 : 4; }
+
+// Tiles and parts of a call.  Unknown lengths are bounded by max_k; block_size
+// 0 (the workspace query does not name one) assumes the smallest, which bounds
+// the parts from above.
+//
+// p parts of the prefix take about A / p + B p us: a unit's steps (1.6 us, 1.0 for
+// tiles of up to 64 rows) against the parts written and read again (1032 bytes a
+// row and head at 3.5 TB/s) and the units' start (5 us over 512 places), where a
+// part costs three times that beside the own keys' units.  Past a unit a CU, as
+// many as fill one or two a CU.  Own keys are cut into parts of about 512 keys, 320
+// where there are few units.  Over 16 shapes (batches of 2-160, 1-64 rows, heads
+// 5/1-64/8, prefixes of 512-16384 keys, bf16 and FP8) timed with all counts of
+// parts the choice is 3% from the best on the geometric mean; a part more or
+// less around it costs little: 64 x 8192 shared keys at 32/8 heads 4 / 6 / 8 / 12 /
+// 16 parts 64 / 52 / 45 / 46 / 53 us, 128 x 8 rows over 4111 at 64/8 heads 1 / 2 / 4
+// 183 / 189 / 194.
+void make_plan(PrefixParams& pp, int32_t prefix_len, int32_t block_size) {
+  AttnParams& p = pp.a;
+  pp.prefix = prefix_len < p.max_k ? prefix_len / 32 * 32 : p.max_k / 32 * 32;
+  p.qtile = kTileRows / p.group;
+  pp.prefix_tiles = ceil_div(p.num_tokens, p.qtile);
+  pp.own_tiles = ceil_div(p.max_q, p.qtile);
+  const int64_t cus = device_cus();
+  const float heads = static_cast<float>(p.num_tokens) * p.hq;
+  const float units = static_cast<float>(pp.prefix_tiles) * p.hkv;   // of one part
+  const float a = (few_rows(p) ? 1.0f : 1.6f) * pp.prefix / kWideKeys;
+  const float b = 3.0f * (heads * 1032.0f / 3.5e6f + units * 5.0f / (2 * cus));
+  float parts = sqrtf(a / b);
+  if (parts * units > cus) {
+    float fill = cus;
+    while (parts * units > 1.41f * fill) fill *= 2.0f;
+    parts = fill / units;
+  }
+  const int32_t most = pp.prefix / (2 * kWideKeys);
+  int32_t count = parts + 0.5f < most ? static_cast<int32_t>(parts + 0.5f) : most;
+  count = count < 1 ? 1 : count;
+  pp.prefix_split = ceil_div(ceil_div(pp.prefix, count), kWideKeys) * kWideKeys;
+  pp.prefix_parts = pp.prefix > 0 ? ceil_div(pp.prefix, pp.prefix_split) : 0;
   // own keys
-  const int32_t own = p.max_k - p.prefix;
-  int64_t own_parts = places / (static_cast<int64_t>(p.num_seqs) * p.own_tiles * p.hkv);
-  const int32_t own_most = own / kMinPart;
-  own_parts = own_parts < 1 ? 1 : own_parts;
-  own_parts = own_parts > own_most ? (own_most < 1 ? 1 : own_most) : own_parts;
-  p.own_split = own > 0 ? ceil_div(ceil_div(own, own_parts), kKeys) * kKeys : kKeys;
-  p.own_parts = own > 0 ? ceil_div(own, p.own_split) : 1;
-  const int64_t prefix_units = static_cast<int64_t>(p.prefix_parts) * p.prefix_tiles;
-  const int64_t own_units = static_cast<int64_t>(p.num_seqs) * p.own_tiles * p.own_parts;
+  const int32_t own = p.max_k - pp.prefix;
+  const int32_t length = static_cast<int64_t>(p.num_seqs) * pp.own_tiles * p.hkv < cus / 2 ? 320 : 512;
+  const int32_t own_count = own / length + (own % length >= length / 2 ? 1 : 0);
+  pp.own_split = own > 0 ? ceil_div(ceil_div(own, own_count < 1 ? 1 : own_count), kWideKeys) * kWideKeys : kWideKeys;
+  // attend_segment holds a part's block ids one a lane
+  const int32_t span = (kWave - 2) * (block_size > 0 ? block_size : kChunk) / kWideKeys * kWideKeys;
+  if (pp.own_split > span) pp.own_split = span;
+  pp.own_parts = own > 0 ? ceil_div(own, pp.own_split) : 1;
+  p.max_splits = pp.prefix_parts + pp.own_parts;
+  const int64_t prefix_units = static_cast<int64_t>(pp.prefix_parts) * pp.prefix_tiles;
+  const int64_t own_units = static_cast<int64_t>(p.num_seqs) * pp.own_tiles * pp.own_parts;
   const bool fits = (prefix_units + own_units) * p.hkv <= 0x7FFFFFFF;
-  p.prefix_units = fits ? static_cast<int32_t>(prefix_units) : -1;
-  p.own_units = fits ? static_cast<int32_t>(own_units) : -1;
+  pp.prefix_units = fits ? static_cast<int32_t>(prefix_units) : -1;
+  pp.own_units = fits ? static_cast<int32_t>(own_units) : -1;
 }
 
-size_t plan_bytes(const PrefixParams& p) {
-  const size_t slots = static_cast<size_t>(p.num_tokens) * p.hq * (p.prefix_parts + p.own_parts);
-  return slots * (kD + 1) * sizeof(float) + static_cast<size_t>(p.num_tokens) * sizeof(int32_t);
+size_t plan_bytes(const PrefixParams& pp) {
+  const size_t slots = static_cast<size_t>(pp.a.num_tokens) * pp.a.hq * pp.a.max_splits;
+  return slots * (kD + 1) * sizeof(float) + static_cast<size_t>(pp.a.num_tokens) * sizeof(int32_t);
 }
 
-int run(PrefixParams& p, int kv_dtype, int32_t prefix_len, void* workspace, size_t workspace_bytes,
+template <int OWN, bool FEW>
+void launch(const PrefixParams& pp, bool fp8, int32_t grid, hipStream_t s) {
+  if (fp8)
+    shared_prefix_kernel<OWN, FEW, true><<<grid, kThreads, 0, s>>>(pp);
+  else
+    shared_prefix_kernel<OWN, FEW, false><<<grid, kThreads, 0, s>>>(pp);
+}
+template <int OWN>
+void launch(const PrefixParams& pp, bool fp8, int32_t grid, hipStream_t s) {
+  if (few_rows(pp.a))
+    launch<OWN, true>(pp, fp8, grid, s);
+  else
+    launch<OWN, false>(pp, fp8, grid, s);
+}
+
+int run(PrefixParams& pp, int kv_dtype, int32_t prefix_len, void* workspace, size_t workspace_bytes,
         hipStream_t s) {
+  AttnParams& p = pp.a;
   if (p.hq <= 0 || p.hkv <= 0 || p.hq % p.hkv != 0) return NVA_ERR_ARG;
   if (kv_dtype != NVA_KV_BF16 && kv_dtype != NVA_KV_FP8_E4M3) return NVA_ERR_ARG;
   if (p.num_seqs < 0 || p.num_tokens < 0 || p.max_q < 0 || p.max_k < 0 || prefix_len < 0) return NVA_ERR_ARG;
@@ -567,20 +581,27 @@ int run(PrefixParams& p, int kv_dtype, int32_t prefix_len, void* workspace, size
       p.q_row_stride % 8 || p.q_head_stride % 8 || p.out_row_stride % 8 || p.out_head_stride % 8 ||
       p.blk_stride % vec || p.tok_stride % vec || p.head_stride % vec)
     return NVA_ERR_UNSUPPORTED;
-  make_plan(p, prefix_len);
-  if (p.own_units < 0) return NVA_ERR_UNSUPPORTED;     // more workgroups than a grid holds
-  if (!workspace || workspace_bytes < plan_bytes(p) || !aligned16(workspace)) return NVA_ERR_WORKSPACE;
-  const size_t slots = static_cast<size_t>(p.num_tokens) * p.hq * (p.prefix_parts + p.own_parts);
+  // the workspace is the query's, which knows no block size
+  make_plan(pp, prefix_len, 0);
+  const size_t need = plan_bytes(pp);
+  make_plan(pp, prefix_len, p.block_size);
+  if (pp.own_units < 0) return NVA_ERR_UNSUPPORTED;    // more workgroups than a grid holds
+  if (!workspace || workspace_bytes < need || workspace_bytes < plan_bytes(pp) || !aligned16(workspace))
+    return NVA_ERR_WORKSPACE;
+  const size_t slots = static_cast<size_t>(p.num_tokens) * p.hq * p.max_splits;
   p.ws_o = static_cast<float*>(workspace);
   p.ws_lse = p.ws_o + slots * kD;
-  p.row_parts = reinterpret_cast<int32_t*>(p.ws_lse + slots);
-  const int32_t grid = p.hkv * (p.prefix_units + p.own_units);
-  if (kv_dtype == NVA_KV_FP8_E4M3)
-    shared_prefix_kernel<kWaves, true><<<grid, kWave * kWaves, 0, s>>>(p);
-  else
-    shared_prefix_kernel<kWaves, false><<<grid, kWave * kWaves, 0, s>>>(p);
+  p.row_nsplit = reinterpret_cast<int32_t*>(p.ws_lse + slots);
+  const int32_t grid = p.hkv * (pp.prefix_units + pp.own_units);
+  const bool fp8 = kv_dtype == NVA_KV_FP8_E4M3;
+  switch (own_kind(static_cast<int64_t>(p.max_q) * p.group)) {
+    case 1: launch<1>(pp, fp8, grid, s); break;
+    case 2: launch<2>(pp, fp8, grid, s); break;
+    case 3: launch<3>(pp, fp8, grid, s); break;
+    default: launch<4>(pp, fp8, grid, s); break;
+  }
   if (hipGetLastError() != hipSuccess) return NVA_ERR_LAUNCH;
-  join_kernel<<<dim3(p.num_tokens, ceil_div(p.hq * (kD / 4), kJoinThreads)), kJoinThreads, 0, s>>>(p);
+  join_kernel<<<dim3(p.num_tokens, ceil_div(p.hq * (kD / 4), kJoinThreads)), kJoinThreads, 0, s>>>(pp);
   return launch_status();
 }
 
@@ -597,7 +618,8 @@ extern "C" size_t nva_shared_prefix_workspace_size(int32_t num_seqs, int32_t num
       max_seqlen_q <= 0 || max_seqlen_k < 0 || prefix_len < 0 || num_q_heads % num_kv_heads ||
       num_q_heads / num_kv_heads > 64)
     return 0;
-  PrefixParams p = {};
+  PrefixParams pp = {};
+  AttnParams& p = pp.a;
   p.num_seqs = num_seqs;
   p.num_tokens = num_tokens;
   p.hq = num_q_heads;
@@ -605,8 +627,8 @@ extern "C" size_t nva_shared_prefix_workspace_size(int32_t num_seqs, int32_t num
   p.group = num_q_heads / num_kv_heads;
   p.max_q = max_seqlen_q;
   p.max_k = max_seqlen_k;
-  make_plan(p, prefix_len);
-  return plan_bytes(p);
+  make_plan(pp, prefix_len, 0);
+  return plan_bytes(pp);
 }
 
 extern "C" int nva_shared_prefix_attention_varlen(
@@ -621,7 +643,8 @@ extern "C" int nva_shared_prefix_attention_varlen(
     void* stream) {
   if (head_dim != kD) return NVA_ERR_UNSUPPORTED;
   if (!cu_seqlens_q || !cu_seqlens_k) return NVA_ERR_ARG;
-  PrefixParams p = {};
+  PrefixParams pp = {};
+  AttnParams& p = pp.a;
   p.q = static_cast<const uint16_t*>(q);
   p.q_row_stride = q_row_stride;
   p.q_head_stride = q_head_stride;
@@ -649,7 +672,7 @@ extern "C" int nva_shared_prefix_attention_varlen(
   p.out = static_cast<uint16_t*>(out);
   p.out_row_stride = out_row_stride;
   p.out_head_stride = out_head_stride;
-  return run(p, kv_dtype, prefix_len, workspace, workspace_bytes, static_cast<hipStream_t>(stream));
+  return run(pp, kv_dtype, prefix_len, workspace, workspace_bytes, static_cast<hipStream_t>(stream));
 }
 
 extern "C" int nva_shared_prefix_attention_decode(
@@ -663,7 +686,8 @@ extern "C" int nva_shared_prefix_attention_decode(
     void* workspace, size_t workspace_bytes, void* stream) {
   if (head_dim != kD) return NVA_ERR_UNSUPPORTED;
   if (!cache_seqlens) return NVA_ERR_ARG;
-  PrefixParams p = {};
+  PrefixParams pp = {};
+  AttnParams& p = pp.a;
   p.q = static_cast<const uint16_t*>(q);
   p.q_row_stride = q_row_stride;
   p.q_head_stride = q_head_stride;
@@ -690,5 +714,5 @@ extern "C" int nva_shared_prefix_attention_decode(
   p.out = static_cast<uint16_t*>(out);
   p.out_row_stride = out_row_stride;
   p.out_head_stride = out_head_stride;
-  return run(p, kv_dtype, prefix_len, workspace, workspace_bytes, static_cast<hipStream_t>(stream));
+  return run(pp, kv_dtype, prefix_len, workspace, workspace_bytes, static_cast<hipStream_t>(stream));
 }
