@@ -10,17 +10,22 @@
 // Scales, the sums of x and the sum over groups are fp32, the output is rounded
 // once.
 //
-// What bounds it: the codes' stream from HBM (a quarter of the bf16 weights').
+// What bounds it: for wide outputs the codes' stream from HBM, a quarter of the
+// bf16 weights' (1 x 151936 x 4096: 58-64 us, 5.0-5.4 TB/s; a 1 GiB copy reaches
+// 5.07).  Below that the start (at 1 x 4096 x 4096, 5.1 us, x is staged 2.1 us
+// into the kernel's 4.1), and from some dozen rows the staging of x and the joining
+// of parts as well (61 x 6144 x 4096 in groups of 32, 21.5 us: staging 5, codes 6,
+// joining waves 4, joining ranges 5).
 //
-// A workgroup of eight waves stages its range of K of all x rows in LDS once,
-// as MFMA operands beside the group sums, and then only streams codes: no
-// barrier, no x traffic in the loop.  WK waves take the steps (256 codes of a
-// row, 128 bytes) of 16 weight rows in turn, 8 / WK times 16 rows a workgroup.
-// A lane's 16 bytes are 32 codes of one row (lane l: row l % 16, codes
-// 32 (l / 16) .. of a 128-wide chunk), four MFMAs deep.  Where groups are
-// shorter than 128 the four lanes of a row exchange dwords (four swaps), so that
-// an MFMA sums over 32 neighbouring codes.  The accumulator's lanes hold one
-// weight row each, so a group costs a lane one scale and one zero: the four
+// A workgroup of eight waves stages its range of K of all x rows in LDS once, as
+// MFMA operands, and then only streams codes: no barrier, no x traffic in the
+// loop (a group's sum of x is a product with ones beside the others).  WK waves
+// take the steps (256 codes of a row, 128 bytes) of 16 weight rows in turn, 8 / WK
+// times 16 rows a workgroup.  A lane's 16 bytes are 32 codes of one row (lane l:
+// row l % 16, codes 32 (l / 16) .. of a 128-wide chunk), four MFMAs deep.  Where
+// groups are shorter than 128 the four lanes of a row exchange dwords (four swaps),
+// so that an MFMA sums over 32 neighbouring codes.  The accumulator's lanes hold
+// one weight row each, so a group costs a lane one scale and one zero: the four
 // lanes of a row load those of four groups and broadcast them by swaps.
 //
 // Ranges of K shared out over workgroups leave fp32 parts that a second kernel
@@ -113,21 +118,13 @@ __device__ __forceinline__ void broadcast(uint32_t (&v)[4]) {
   swap16(v[2], v[3]);
 }
 
-// LDS of a step: x rows of two chunks, then the sums of x over its groups.
-template <int RT, int PER>
-struct Step {
-  static constexpr int kGroups = 8 / PER;
-  static constexpr int kDwords = 2 * RT * kXPitch + kGroups * RT;
-};
-
 // RT: rows of x staged; PER: MFMAs (32 codes each) per group, 1, 2 or 4 (whole
 // chunks); NT: tiles of 16 weight rows of a wave; D: steps in flight; WK: waves
 // that share a tile.
 template <int RT, int PER, int NT, int D, int WK>
 __global__ void __launch_bounds__(kThreads, RT <= 16 ? 4 : 2) linear_w4_kernel(W4Params p) {
-  using S = Step<RT, PER>;
   constexpr int MT = RT <= 16 ? 1 : RT / 16;           // tiles of 16 rows of x
-  constexpr int kGroups = S::kGroups;
+  constexpr int kGroups = 8 / PER;                     // of a step
   constexpr int kLoads = (kGroups + 3) / 4;            // of a lane's scales per step
   extern __shared__ __attribute__((aligned(16))) uint32_t xs[];
   const int lane = threadIdx.x & (kWave - 1);
@@ -187,65 +184,59 @@ __global__ void __launch_bounds__(kThreads, RT <= 16 ? 4 : 2) linear_w4_kernel(W
     }
   };
 
-  Codes buf[D];
-#pragma unroll
-  for (int d = 0; d < D; ++d)
-    if (mine + d * WK < end) load(mine + d * WK, buf[d]);
-
-  // ---- x of this range, once: piece i is 16 bytes, sixteen lanes a chunk's row;
-  // a batch of loads is in flight at a time
-  constexpr int kBatch = 4;
+  // ---- x of this range, once: piece i is 16 bytes, sixteen lanes a chunk's row.
+  // The first batch is asked for before the codes: loads return in order, and x
+  // comes from L2 in half the time that the codes take from HBM.
+  constexpr int kBatch = RT <= 16 ? 8 : 16;
   const int pieces = (end - first) * 2 * RT * 16;
-  for (int i0 = threadIdx.x; i0 < pieces; i0 += kBatch * blockDim.x) {
-    uint4 v[kBatch];
+  uint4 xv[kBatch];
+  auto load_x = [&](int i0) {
 #pragma unroll
     for (int u = 0; u < kBatch; ++u) {
       const int i = i0 + u * blockDim.x;
       const int xr = (i / 16) % RT, k = first * kStepK + i / (16 * RT) * kChunkK + 8 * m16;
-      v[u] = make_uint4(0, 0, 0, 0);
+      xv[u] = make_uint4(0, 0, 0, 0);
       if (i < pieces && xr < M && k < p.K)
-        v[u] = *reinterpret_cast<const uint4*>(p.x + static_cast<int64_t>(m0 + xr) * p.x_stride + k);
+        xv[u] = *reinterpret_cast<const uint4*>(p.x + static_cast<int64_t>(m0 + xr) * p.x_stride + k);
     }
+  };
+  auto stage_x = [&](int i0) {
 #pragma unroll
     for (int u = 0; u < kBatch; ++u) {
       const int i = i0 + u * blockDim.x;
       const int xr = (i / 16) % RT, chunk = i / (16 * RT);
       if (i < pieces)
-        *reinterpret_cast<uint4*>(xs + (chunk / 2) * S::kDwords + ((chunk & 1) * RT + xr) * kXPitch + 4 * m16) =
-            as_operand(v[u]);
+        *reinterpret_cast<uint4*>(xs + (chunk * RT + xr) * kXPitch + 4 * m16) = as_operand(xv[u]);
     }
-  }
-  __syncthreads();
-  const int xrow = RT < 16 ? m16 & (RT - 1) : m16;     // an operand row that is not staged repeats one that is
-  const int srow = RT < 16 ? (4 * g) & (RT - 1) : 4 * g;
-  // the sums of x over each group, by products with ones: every lane of quarter
-  // g holds those of rows 4 g ..
-  const bf16x8_t ones = __builtin_bit_cast(bf16x8_t, make_uint4(0x3F803F80u, 0x3F803F80u, 0x3F803F80u, 0x3F803F80u));
-  for (int i = wv; i < (end - first) * kGroups * MT; i += waves) {
-    const int m = i % MT, grp = i / MT % kGroups;
-    uint32_t* step = xs + i / (MT * kGroups) * S::kDwords;
-    f32x4_t sum = f32x4_t{0.f, 0.f, 0.f, 0.f};
+  };
+  load_x(threadIdx.x);
+  __builtin_amdgcn_sched_barrier(0);
+  Codes buf[D];
 #pragma unroll
-    for (int d = 0; d < PER; ++d) {
-      const int part = grp * PER + d;                  // of the step's eight
-      sum = __builtin_amdgcn_mfma_f32_16x16x32_bf16(
-          *reinterpret_cast<const bf16x8_t*>(step + (part / 4 * RT + 16 * m + xrow) * kXPitch + 16 * (part % 4) + 4 * g),
-          ones, sum, 0, 0, 0);
-    }
-    if (m16 == 0 && 4 * g < RT)
-      *reinterpret_cast<f32x4_t*>(step + 2 * RT * kXPitch + grp * RT + 16 * m + 4 * g) = sum;
+  for (int d = 0; d < D; ++d)
+    if (mine + d * WK < end) load(mine + d * WK, buf[d]);
+  __builtin_amdgcn_sched_barrier(0);
+  stage_x(threadIdx.x);
+  for (int i0 = threadIdx.x + kBatch * blockDim.x; i0 < pieces; i0 += kBatch * blockDim.x) {
+    load_x(i0);
+    stage_x(i0);
   }
   __syncthreads();
 
+  const int xrow = RT < 16 ? m16 & (RT - 1) : m16;     // an operand row that is not staged repeats one that is
+  const bf16x8_t ones = __builtin_bit_cast(bf16x8_t, make_uint4(0x3F803F80u, 0x3F803F80u, 0x3F803F80u, 0x3F803F80u));
   const CodeBits bits;
   f32x4_t acc[NT][MT];
 #pragma unroll
   for (int q = 0; q < NT; ++q)
 #pragma unroll
     for (int m = 0; m < MT; ++m) acc[q][m] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+  const f32x4_t none = f32x4_t{0.f, 0.f, 0.f, 0.f};
+  // TU chunks of a step side by side, where registers allow: their chains of
+  // products are independent
+  constexpr int TU = MT == 1 ? 2 : 1;
   auto compute = [&](int c, const Codes& b) {
-    const uint32_t* step = xs + (c - first) * S::kDwords;
-    const float* xsum = reinterpret_cast<const float*>(step + 2 * RT * kXPitch);
+    const uint32_t* step = xs + (c - first) * 2 * RT * kXPitch;
     uint32_t sz[NT][4 * kLoads];                       // scale (low half) and zero of each group
 #pragma unroll
     for (int q = 0; q < NT; ++q)
@@ -262,42 +253,52 @@ __global__ void __launch_bounds__(kThreads, RT <= 16 ? 4 : 2) linear_w4_kernel(W
         for (int j = 0; j < 4; ++j) sz[q][4 * i + j] = v[j];
       }
 #pragma unroll
-    for (int t = 0; t < 2; ++t) {
-      uint32_t w[NT][4];
+    for (int t0 = 0; t0 < 2; t0 += TU) {
+      uint32_t w[NT][TU][4];
 #pragma unroll
-      for (int q = 0; q < NT; ++q) {
-        w[q][0] = b.w[q][t].x; w[q][1] = b.w[q][t].y; w[q][2] = b.w[q][t].z; w[q][3] = b.w[q][t].w;
-        if constexpr (PER < 4) transpose(w[q]);
-      }
-      f32x4_t sum[NT][MT];
+      for (int q = 0; q < NT; ++q)
+#pragma unroll
+        for (int t = 0; t < TU; ++t) {
+          const uint4 v = b.w[q][t0 + t];
+          w[q][t][0] = v.x; w[q][t][1] = v.y; w[q][t][2] = v.z; w[q][t][3] = v.w;
+          if constexpr (PER < 4) transpose(w[q][t]);
+        }
+      f32x4_t sum[TU][NT][MT], xsum[TU][MT];           // of a group: codes by x, and x
 #pragma unroll
       for (int d = 0; d < 4; ++d) {
-        bf16x8_t wo[NT];
 #pragma unroll
-        for (int q = 0; q < NT; ++q) wo[q] = bits.operand(w[q][d]);
+        for (int t = 0; t < TU; ++t) {
+          bf16x8_t wo[NT];
 #pragma unroll
-        for (int m = 0; m < MT; ++m) {
-          const bf16x8_t xo = *reinterpret_cast<const bf16x8_t*>(
-              step + (t * RT + 16 * m + xrow) * kXPitch + (PER < 4 ? 16 * d + 4 * g : 16 * g + 4 * d));
-#pragma unroll
-          for (int q = 0; q < NT; ++q)
-            sum[q][m] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(
-                xo, wo[q], d % PER == 0 ? f32x4_t{0.f, 0.f, 0.f, 0.f} : sum[q][m], 0, 0, 0);
-        }
-        if (d % PER == PER - 1) {
-          const int i = t * (4 / PER) + d / PER;
+          for (int q = 0; q < NT; ++q) wo[q] = bits.operand(w[q][t][d]);
 #pragma unroll
           for (int m = 0; m < MT; ++m) {
-            const f32x4_t x1 = *reinterpret_cast<const f32x4_t*>(xsum + i * RT + 16 * m + srow);
+            const bf16x8_t xo = *reinterpret_cast<const bf16x8_t*>(
+                step + ((t0 + t) * RT + 16 * m + xrow) * kXPitch + (PER < 4 ? 16 * d + 4 * g : 16 * g + 4 * d));
+            xsum[t][m] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(xo, ones, d % PER == 0 ? none : xsum[t][m], 0, 0, 0);
+#pragma unroll
+            for (int q = 0; q < NT; ++q)
+              sum[t][q][m] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(
+                  xo, wo[q], d % PER == 0 ? none : sum[t][q][m], 0, 0, 0);
+          }
+        }
+        if (d % PER == PER - 1) {
+#pragma unroll
+          for (int t = 0; t < TU; ++t) {
+            const int i = (t0 + t) * (4 / PER) + d / PER;
 #pragma unroll
             for (int q = 0; q < NT; ++q) {
               const float s = __uint_as_float(sz[q][i] << 16), z = 16.0f + static_cast<float>(sz[q][i] >> 16);
 #pragma unroll
-              for (int e = 0; e < 4; ++e)
-                acc[q][m][e] = __builtin_fmaf(s, __builtin_fmaf(-z, x1[e], sum[q][m][e]), acc[q][m][e]);
-              // the sums so far are wanted here: put off to the end of the step,
-              // the operands of all its groups stay in registers and spill
-              asm("" : "+v"(acc[q][m]));
+              for (int m = 0; m < MT; ++m) {
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+                  acc[q][m][e] =
+                      __builtin_fmaf(s, __builtin_fmaf(-z, xsum[t][m][e], sum[t][q][m][e]), acc[q][m][e]);
+                // the sums so far are wanted here: put off to the end of the
+                // step, the operands of all its groups stay in registers and spill
+                asm("" : "+v"(acc[q][m]));
+              }
             }
           }
         }
@@ -314,7 +315,7 @@ __global__ void __launch_bounds__(kThreads, RT <= 16 ? 4 : 2) linear_w4_kernel(W
   }
 
   if constexpr (WK > 1) {
-    // the waves of a tile meet in LDS, in wave order (deterministic)
+    // the waves of a tile meet in LDS and are summed in wave order (deterministic)
     __syncthreads();
     f32x4_t* const sums = reinterpret_cast<f32x4_t*>(xs);
 #pragma unroll
@@ -322,50 +323,65 @@ __global__ void __launch_bounds__(kThreads, RT <= 16 ? 4 : 2) linear_w4_kernel(W
 #pragma unroll
       for (int m = 0; m < MT; ++m) sums[((wv * NT + q) * MT + m) * kWave + lane] = acc[q][m];
     __syncthreads();
-    if (wv % WK != 0) return;
-#pragma unroll
-    for (int q = 0; q < NT; ++q)
-#pragma unroll
-      for (int m = 0; m < MT; ++m)
-#pragma unroll
-        for (int v = 1; v < WK; ++v) {
-          const f32x4_t a = sums[(((wv + v) * NT + q) * MT + m) * kWave + lane];
-#pragma unroll
-          for (int e = 0; e < 4; ++e) acc[q][m][e] += a[e];
-        }
   }
 
-  // a lane's columns n of four rows
+  // a lane's column n of four rows; the tiles of 16 x 16 are dealt to the waves
+  // that share them
 #pragma unroll
-  for (int q = 0; q < NT; ++q) {
+  for (int qm = 0; qm < NT * MT; ++qm) {
+    const int q = qm / MT, m = qm % MT;
+    f32x4_t sum = acc[q][m];
+    if constexpr (WK > 1) {
+      if (qm % WK != wv % WK) continue;
+      const f32x4_t* at = reinterpret_cast<const f32x4_t*>(xs) + ((wv / WK * WK) * NT * MT + qm) * kWave + lane;
+      sum = at[0];
+#pragma unroll
+      for (int v = 1; v < WK; ++v) {
+        const f32x4_t a = at[v * NT * MT * kWave];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) sum[e] += a[e];
+      }
+    }
     const int n = n0 + 16 * q + m16;
-    if (n >= p.N) return;
+    if (n >= p.N) continue;
     const float bias = !p.partial && p.bias ? bf16_to_f32(p.bias[n]) : 0.0f;
 #pragma unroll
-    for (int m = 0; m < MT; ++m)
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const int r = 16 * m + 4 * g + e;
-        if (r >= M) continue;
-        if (p.partial)
-          p.partial[(static_cast<int64_t>(split) * p.M + m0 + r) * p.N + n] = acc[q][m][e];
-        else
-          p.out[static_cast<int64_t>(m0 + r) * p.out_stride + n] = f32_to_bf16(acc[q][m][e] + bias);
-      }
+    for (int e = 0; e < 4; ++e) {
+      const int r = 16 * m + 4 * g + e;
+      if (r >= M) continue;
+      if (p.partial)
+        p.partial[(static_cast<int64_t>(split) * p.M + m0 + r) * p.N + n] = sum[e];
+      else
+        p.out[static_cast<int64_t>(m0 + r) * p.out_stride + n] = f32_to_bf16(sum[e] + bias);
+    }
   }
 }
 
-// The sum of the K ranges' parts, in order.
+// The sum of the K ranges' parts, in order: a thread owns V columns of a row and
+// loads kSumBatch parts at a time (one latency, not one a part).
+constexpr int kSumBatch = 8;
+template <int V>
 __global__ void __launch_bounds__(256) linear_w4_sum_kernel(W4Params p, int32_t splits) {
+  typedef __attribute__((ext_vector_type(V))) float vec;
   const int64_t i = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x;
-  const int64_t size = static_cast<int64_t>(p.M) * p.N;
+  const int64_t size = static_cast<int64_t>(p.M) * p.N / V;
   if (i >= size) return;
-  const int64_t m = i / p.N;
-  const int n = static_cast<int>(i - m * p.N);
-  float s = p.partial[i];
-  for (int j = 1; j < splits; ++j) s += p.partial[j * size + i];
-  if (p.bias) s += bf16_to_f32(p.bias[n]);
-  p.out[m * p.out_stride + n] = f32_to_bf16(s);
+  const int64_t m = i / (p.N / V);
+  const int n = static_cast<int>(i - m * (p.N / V)) * V;
+  const vec* part = reinterpret_cast<const vec*>(p.partial) + i;
+  vec s = 0.0f;
+  for (int j0 = 0; j0 < splits; j0 += kSumBatch) {
+    vec a[kSumBatch];
+#pragma unroll
+    for (int u = 0; u < kSumBatch; ++u) a[u] = j0 + u < splits ? part[(j0 + u) * size] : vec(0.0f);
+#pragma unroll
+    for (int u = 0; u < kSumBatch; ++u)
+#pragma unroll
+      for (int e = 0; e < V; ++e) s[e] += a[u][e];
+  }
+  uint16_t* o = p.out + m * p.out_stride + n;
+#pragma unroll
+  for (int e = 0; e < V; ++e) o[e] = f32_to_bf16(p.bias ? s[e] + bf16_to_f32(p.bias[n + e]) : s[e]);
 }
 
 // Rows of x a workgroup stages, ranges of K, waves of a workgroup, and how many of
@@ -380,7 +396,7 @@ constexpr int tiles_of(int rt) { return rt <= 16 ? 1 : 2; }
 template <int RT, int PER, int NT, int D, int WK>
 int launch(const W4Params& p, const W4Plan& plan, hipStream_t s) {
   const int steps = ((p.K + kStepK - 1) / kStepK + plan.splits - 1) / plan.splits;
-  int bytes = steps * Step<RT, PER>::kDwords * 4;
+  int bytes = steps * 2 * RT * kXPitch * 4;
   const int sums = plan.waves * kWave * NT * (RT <= 16 ? 1 : RT / 16) * 16;
   if (WK > 1 && bytes < sums) bytes = sums;
   const int tile = 16 * NT * (plan.waves / WK);
@@ -445,16 +461,20 @@ W4Plan make_plan(int32_t rows, int32_t n, int32_t k, int32_t group) {
   best.waves = kWaves;
   const int rt = best.rows, nt = tiles_of(rt), mt = rt <= 16 ? 1 : rt / 16;
   const int per = group % 128 == 0 ? 4 : group % 64 == 0 ? 2 : 1;
-  const int step_bytes = (2 * rt * kXPitch + 8 / per * rt) * 4;
+  const int step_bytes = 2 * rt * kXPitch * 4;
   const int32_t steps = (k + kStepK - 1) / kStepK, most = kMaxLds / step_bytes;
   const int64_t cus = device_cus(), slabs = (rows + 63) / 64;
-  const float unit = 0.59f * nt * (1.0f + 0.35f * (mt - 1)) * (1.0f + 0.33f * (4 / per - 1));
+  const float unit = 0.53f * nt * (1.0f + 0.22f * (mt - 1)) * (1.0f + 0.23f * (4 / per - 1));
   const int slots = rt <= 16 ? 2 : 1;                  // workgroups of a CU by registers
   float least = 0.0f;
   for (int shared = 1; shared <= kWaves; shared *= 2) {
     const int tile = 16 * nt * (kWaves / shared);
     const int64_t tiles = (n + tile - 1) / tile * slabs;
-    for (int32_t splits = (steps + most - 1) / most; splits <= steps; ++splits) {
+    const int32_t fewest = (steps + most - 1) / most;
+    for (int fill = 0; fill <= 4; fill = fill ? 2 * fill : 1) {
+      // as few ranges as LDS allows, or as many as make one, two, four rounds
+      int32_t splits = fill ? static_cast<int32_t>(fill * cus / tiles) : fewest;
+      if (splits < fewest || (fill && splits == fewest) || splits > steps) continue;
       const int32_t of_range = (steps + splits - 1) / splits;
       int bytes = of_range * step_bytes;
       const int parked = kThreads * nt * mt * 16;
@@ -463,18 +483,21 @@ W4Plan make_plan(int32_t rows, int32_t n, int32_t k, int32_t group) {
       const int64_t per_cu = (tiles * splits + cus - 1) / cus;
       const int64_t at_once = per_cu < fit ? per_cu : fit;
       float t = unit * ((of_range + shared - 1) / shared) * (at_once > 1 ? at_once : 1.0f) +
-                0.016f * of_range * rt + (shared > 1 ? 0.018f * nt * mt * shared : 0.0f);
+                0.014f * of_range * rt + (shared > 1 ? 0.012f * nt * mt * shared : 0.0f);
       t *= static_cast<float>((per_cu + at_once - 1) / at_once);
-      if (splits > 1) t += 2.5f + 2.5e-6f * splits * rows * n;
+      if (splits > 1) t += 2.3f + 2.8e-6f * splits * rows * n;
       if (best.splits == 0 || t < least) {
         least = t;
         best.splits = splits;
         best.shared = shared;
       }
-      if (tiles * splits > 4 * cus) break;             // more ranges only cost
     }
   }
   return best;
+}
+
+size_t plan_bytes(const W4Plan& w, int32_t rows, int32_t n) {
+  return w.splits > 1 ? static_cast<size_t>(w.splits) * rows * n * sizeof(float) : 0;
 }
 
 }  // namespace
@@ -484,8 +507,7 @@ using namespace nva;
 
 extern "C" size_t nva_linear_w4_workspace_size(int32_t rows, int32_t n, int32_t k, int32_t group) {
   if (rows <= 0 || n <= 0 || k <= 0 || group <= 0 || k % group || group % 32) return 0;
-  const W4Plan w = make_plan(rows, n, k, group);
-  return w.splits > 1 ? static_cast<size_t>(w.splits) * rows * n * sizeof(float) : 0;
+  return plan_bytes(make_plan(rows, n, k, group), rows, n);
 }
 
 extern "C" int nva_linear_w4(const void* x, int64_t x_row_stride, const void* qweight,
@@ -502,7 +524,7 @@ extern "C" int nva_linear_w4(const void* x, int64_t x_row_stride, const void* qw
       k > (1 << 20) || static_cast<int64_t>(k / group) * n >= 1 << 29)
     return NVA_ERR_UNSUPPORTED;
   const W4Plan plan = make_plan(rows, n, k, group);
-  const size_t need = nva_linear_w4_workspace_size(rows, n, k, group);
+  const size_t need = plan_bytes(plan, rows, n);
   if (need && (!workspace || workspace_bytes < need || !aligned16(workspace))) return NVA_ERR_WORKSPACE;
   const W4Params p{static_cast<const uint16_t*>(x), x_row_stride, static_cast<const uint8_t*>(qweight),
                    static_cast<const uint16_t*>(scales), static_cast<const uint8_t*>(zeros),
@@ -520,7 +542,8 @@ extern "C" int nva_linear_w4(const void* x, int64_t x_row_stride, const void* qw
     default: status = launch_shared<64>(p, plan, s); break;
   }
   if (status != NVA_OK || plan.splits == 1) return status;
-  const int64_t size = static_cast<int64_t>(rows) * n;
-  linear_w4_sum_kernel<<<static_cast<uint32_t>((size + 255) / 256), 256, 0, s>>>(p, plan.splits);
+  const int64_t threads = static_cast<int64_t>(rows) * n / (n % 4 == 0 ? 4 : 1);
+  auto* sum = n % 4 == 0 ? linear_w4_sum_kernel<4> : linear_w4_sum_kernel<1>;
+  sum<<<static_cast<uint32_t>((threads + 255) / 256), 256, 0, s>>>(p, plan.splits);
   return launch_status();
 }
