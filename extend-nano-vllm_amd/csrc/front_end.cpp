@@ -586,6 +586,7 @@ PyObject* linear_w4(PyObject*, PyObject* const* v, Py_ssize_t n) {
       bias = b.data_ptr();
     }
     need(x.stride(0) >= k && x.stride(0) % 8 == 0 && reinterpret_cast<uintptr_t>(x.data_ptr()) % 16 == 0);
+    need(rows <= 16 || x.stride(0) < (1 << 24));
     at::Tensor out;
     if (a.none(5)) {
       out = empty_bf16({rows, m}, x);

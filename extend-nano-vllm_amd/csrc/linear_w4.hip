@@ -13,20 +13,26 @@
 // What bounds it: for wide outputs the codes' stream from HBM, a quarter of the
 // bf16 weights' (1 x 151936 x 4096: 58-64 us, 5.0-5.4 TB/s; a 1 GiB copy reaches
 // 5.07).  Below that the start (at 1 x 4096 x 4096, 5.1 us, x is staged 2.1 us
-// into the kernel's 4.1), and from some dozen rows the staging of x and the joining
-// of parts as well (61 x 6144 x 4096 in groups of 32, 21.5 us: staging 5, codes 6,
-// joining waves 4, joining ranges 5).
+// into the kernel's 4.1).  From some dozen rows on a step's work, products, codes
+// to operands, scales and x through LDS, each about a quarter of its time (64 x
+// 24576 x 4096, 37 us: matrix and vector units busy 34% and 31% of the cycles).
 //
-// A workgroup of eight waves stages its range of K of all x rows in LDS once, as
-// MFMA operands, and then only streams codes: no barrier, no x traffic in the
-// loop (a group's sum of x is a product with ones beside the others).  WK waves
-// take the steps (256 codes of a row, 128 bytes) of 16 weight rows in turn, 8 / WK
-// times 16 rows a workgroup.  A lane's 16 bytes are 32 codes of one row (lane l:
-// row l % 16, codes 32 (l / 16) .. of a 128-wide chunk), four MFMAs deep.  Where
-// groups are shorter than 128 the four lanes of a row exchange dwords (four swaps),
-// so that an MFMA sums over 32 neighbouring codes.  The accumulator's lanes hold
-// one weight row each, so a group costs a lane one scale and one zero: the four
-// lanes of a row load those of four groups and broadcast them by swaps.
+// Codes come to the waves in steps: 256 codes of each of 16 rows, 128 bytes of a
+// row.  A lane's 16 bytes are 32 codes of one row (lane l: row l % 16, codes
+// 32 (l / 16) .. of a 128-wide chunk), four MFMAs deep.  Where groups are shorter
+// than 128 the four lanes of a row exchange dwords (four swaps), so that an MFMA
+// sums over 32 neighbouring codes.  The accumulator's lanes hold one weight row
+// each, so a group costs a lane one scale and one zero: the four lanes of a row
+// load those of four groups and broadcast them by swaps.  WK of a workgroup's eight
+// waves take a tile's steps in turn and meet in LDS.
+//
+// Up to 16 rows a workgroup stages its range of K of all x rows in LDS once, as
+// MFMA operands, and then only streams codes: no barrier, no x traffic in the loop
+// (a group's sum of x is a product with ones beside the others).  More rows would
+// leave room for short ranges only, whose staging and joining took most of the time
+// (61 x 6144 x 4096 21.5 us, 64 x 24576 x 4096 45); there x passes through LDS in
+// chunks of 128 (17.7 and 37 us).  For up to 16 rows the chunks are the slower form
+// where N is wide (16 x 24576 x 4096 18.8 us against 17.9).
 //
 // Ranges of K shared out over workgroups leave fp32 parts that a second kernel
 // sums in order.
@@ -118,52 +124,46 @@ __device__ __forceinline__ void broadcast(uint32_t (&v)[4]) {
   swap16(v[2], v[3]);
 }
 
-// RT: rows of x staged; PER: MFMAs (32 codes each) per group, 1, 2 or 4 (whole
-// chunks); NT: tiles of 16 weight rows of a wave; D: steps in flight; WK: waves
-// that share a tile.
-template <int RT, int PER, int NT, int D, int WK>
-__global__ void __launch_bounds__(kThreads, RT <= 16 ? 4 : 2) linear_w4_kernel(W4Params p) {
-  constexpr int MT = RT <= 16 ? 1 : RT / 16;           // tiles of 16 rows of x
-  constexpr int kGroups = 8 / PER;                     // of a step
-  constexpr int kLoads = (kGroups + 3) / 4;            // of a lane's scales per step
-  extern __shared__ __attribute__((aligned(16))) uint32_t xs[];
-  const int lane = threadIdx.x & (kWave - 1);
-  const int wv = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
-  const int m16 = lane & 15, g = lane >> 4;
-  const int waves = blockDim.x / kWave;
-  const int n0 = blockIdx.x * (16 * NT * (waves / WK)) + 16 * NT * (wv / WK);
-  const int split = blockIdx.y;
-  const int m0 = blockIdx.z * 64;
-  const int M = p.M - m0 < 64 ? p.M - m0 : 64;
-  const int nsteps = (p.K + kStepK - 1) / kStepK;
-  const int first = static_cast<int>(static_cast<int64_t>(nsteps) * split / gridDim.y);
-  const int end = static_cast<int>(static_cast<int64_t>(nsteps) * (split + 1) / gridDim.y);
-  const int mine = first + wv % WK;
-
-  // rows past the end repeat the last one; what they give is not stored.  Loads
-  // go through descriptors that end with their array (the whole offset in the
-  // lane's, which alone is checked): past the end of K x is zero and the codes
-  // are any (the next row's, or zeros past the last), and past the last group
-  // scales are zero.
-  const int top = n0 < p.N ? n0 : p.N - 1;
-  const int64_t base = static_cast<int64_t>(top) * (p.K / 2);
-  const int64_t rest = static_cast<int64_t>(p.N) * (p.K / 2) - base;
-  const __amdgpu_buffer_rsrc_t wr = make_rsrc(p.w + base, rest < 0x7FFFFFFF ? static_cast<int>(rest) : 0x7FFFFFFF);
-  int row[NT], woff[NT];
-#pragma unroll
-  for (int q = 0; q < NT; ++q) {
-    row[q] = n0 + 16 * q + m16 < p.N ? n0 + 16 * q + m16 : p.N - 1;
-    woff[q] = (row[q] - top) * (p.K / 2) + 16 * g;
-  }
-  const int codes_of_zeros = static_cast<int>(p.groups * p.N);
-  const __amdgpu_buffer_rsrc_t sr = make_rsrc(p.scales, 2 * codes_of_zeros);
-  const __amdgpu_buffer_rsrc_t zr = make_rsrc(p.zeros, codes_of_zeros);
-  const bool straight = p.per_group == PER;            // a group is what an accumulator sums
-  struct Codes {
+// What a wave streams: the steps of NT times 16 weight rows from row n0, groups of
+// PER products (32 codes each; 4 also where a group is several).  Rows past the end
+// repeat the last one; what they give is not stored.  Loads go through descriptors
+// that end with their array (the whole offset in the lane's, which alone is
+// checked): past the end of K the codes are any (the next row's, or zeros past the
+// last), and past the last group scales are zero.
+template <int PER, int NT>
+struct CodeStream {
+  static constexpr int kGroups = 8 / PER;              // of a step
+  static constexpr int kLoads = (kGroups + 3) / 4;     // of a lane's scales per step
+  struct Step {
     uint4 w[NT][2];
     uint32_t s[NT][kLoads], z[NT][kLoads];
   };
-  auto load = [&](int c, Codes& b) {
+  __amdgpu_buffer_rsrc_t wr, sr, zr;
+  int row[NT], woff[NT], n, g;
+  uint32_t magic;
+  bool straight, zeros;                                // a group is what an accumulator sums
+
+  __device__ __forceinline__ CodeStream(const W4Params& p, int n0, int lane) {
+    const int top = n0 < p.N ? n0 : p.N - 1;
+    const int64_t base = static_cast<int64_t>(top) * (p.K / 2);
+    const int64_t rest = static_cast<int64_t>(p.N) * (p.K / 2) - base;
+    wr = make_rsrc(p.w + base, rest < 0x7FFFFFFF ? static_cast<int>(rest) : 0x7FFFFFFF);
+    const int scales = static_cast<int>(p.groups * p.N);
+    sr = make_rsrc(p.scales, 2 * scales);
+    zr = make_rsrc(p.zeros, scales);
+    n = p.N;
+    g = lane >> 4;
+#pragma unroll
+    for (int q = 0; q < NT; ++q) {
+      row[q] = n0 + 16 * q + (lane & 15) < n ? n0 + 16 * q + (lane & 15) : n - 1;
+      woff[q] = (row[q] - top) * (p.K / 2) + 16 * g;
+    }
+    magic = p.group_magic;
+    straight = p.per_group == PER;
+    zeros = p.zeros != nullptr;
+  }
+
+  __device__ __forceinline__ void load(int c, Step& b) const {
 #pragma unroll
     for (int q = 0; q < NT; ++q)
 #pragma unroll
@@ -174,36 +174,99 @@ __global__ void __launch_bounds__(kThreads, RT <= 16 ? 4 : 2) linear_w4_kernel(W
 #pragma unroll
     for (int i = 0; i < kLoads; ++i) {
       const int j = kGroups < 4 ? g % kGroups : 4 * i + g;
-      int at = j * p.N + kGroups * c * p.N;
-      if (!straight) at = static_cast<int>(__umulhi(8 * c + PER * j, p.group_magic)) * p.N;
+      int at = j * n + kGroups * c * n;
+      if (!straight) at = static_cast<int>(__umulhi(8 * c + PER * j, magic)) * n;
 #pragma unroll
       for (int q = 0; q < NT; ++q) {
         b.s[q][i] = __builtin_amdgcn_raw_buffer_load_b16(sr, 2 * (at + row[q]), 0, 0);
-        b.z[q][i] = p.zeros ? __builtin_amdgcn_raw_buffer_load_b8(zr, at + row[q], 0, 0) : 8;
+        b.z[q][i] = zeros ? __builtin_amdgcn_raw_buffer_load_b8(zr, at + row[q], 0, 0) : 8;
       }
     }
-  };
+  }
+};
 
-  // ---- x of this range, once: piece i is 16 bytes, sixteen lanes a chunk's row.
-  // The first batch is asked for before the codes: loads return in order, and x
-  // comes from L2 in half the time that the codes take from HBM.
-  constexpr int kBatch = RT <= 16 ? 8 : 16;
+// Adds up the WK waves of a tile in wave order, through LDS that holds nothing any
+// wave still reads, and stores the rows m0 .. m0 + M: a lane has column n0 + 16 q +
+// l % 16 of four rows.  The tiles of 16 x 16 are dealt to the waves that share them.
+template <int NT, int MT, int WK>
+__device__ __forceinline__ void store_tiles(const W4Params& p, const f32x4_t (&acc)[NT][MT], uint32_t* lds, int wv,
+                                            int lane, int n0, int split, int m0, int M) {
+  f32x4_t* const sums = reinterpret_cast<f32x4_t*>(lds);
+  if constexpr (WK > 1) {
+#pragma unroll
+    for (int q = 0; q < NT; ++q)
+#pragma unroll
+      for (int m = 0; m < MT; ++m) sums[((wv * NT + q) * MT + m) * kWave + lane] = acc[q][m];
+    __syncthreads();
+  }
+#pragma unroll
+  for (int qm = 0; qm < NT * MT; ++qm) {
+    const int q = qm / MT, m = qm % MT;
+    f32x4_t sum = acc[q][m];
+    if constexpr (WK > 1) {
+      if (qm % WK != wv % WK) continue;
+      const f32x4_t* at = sums + ((wv / WK * WK) * NT * MT + qm) * kWave + lane;
+      sum = at[0];
+#pragma unroll
+      for (int v = 1; v < WK; ++v) {
+        const f32x4_t a = at[v * NT * MT * kWave];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) sum[e] += a[e];
+      }
+    }
+    const int n = n0 + 16 * q + (lane & 15);
+    if (n >= p.N) continue;
+    const float bias = !p.partial && p.bias ? bf16_to_f32(p.bias[n]) : 0.0f;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const int r = 16 * m + 4 * (lane >> 4) + e;
+      if (r >= M) continue;
+      if (p.partial)
+        p.partial[(static_cast<int64_t>(split) * p.M + m0 + r) * p.N + n] = sum[e];
+      else
+        p.out[static_cast<int64_t>(m0 + r) * p.out_stride + n] = f32_to_bf16(sum[e] + bias);
+    }
+  }
+}
+
+// Up to 16 rows of x, RT of them staged; WK waves share a tile of 16 weight rows.
+template <int RT, int PER, int WK>
+__global__ void __launch_bounds__(kThreads, 4) linear_w4_kernel(W4Params p) {
+  using Stream = CodeStream<PER, 1>;
+  constexpr int D = 3;                                 // steps in flight
+  constexpr int kGroups = Stream::kGroups, kLoads = Stream::kLoads;
+  extern __shared__ __attribute__((aligned(16))) uint32_t xs[];
+  const int lane = threadIdx.x & (kWave - 1);
+  const int wv = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
+  const int m16 = lane & 15, g = lane >> 4;
+  const int n0 = 16 * (blockIdx.x * (kWaves / WK) + wv / WK);
+  const int nsteps = (p.K + kStepK - 1) / kStepK;
+  const int first = static_cast<int>(static_cast<int64_t>(nsteps) * blockIdx.y / gridDim.y);
+  const int end = static_cast<int>(static_cast<int64_t>(nsteps) * (blockIdx.y + 1) / gridDim.y);
+  const int mine = first + wv % WK;
+  const Stream codes(p, n0, lane);
+
+  // ---- x of this range, once: piece i is 16 bytes, sixteen lanes a chunk's row,
+  // zeros past the end of K.  The first batch is asked for before the codes: loads
+  // return in order, and x comes from L2 in half the time that the codes take from
+  // HBM.
+  constexpr int kBatch = 8;
   const int pieces = (end - first) * 2 * RT * 16;
   uint4 xv[kBatch];
   auto load_x = [&](int i0) {
 #pragma unroll
     for (int u = 0; u < kBatch; ++u) {
-      const int i = i0 + u * blockDim.x;
+      const int i = i0 + u * kThreads;
       const int xr = (i / 16) % RT, k = first * kStepK + i / (16 * RT) * kChunkK + 8 * m16;
       xv[u] = make_uint4(0, 0, 0, 0);
-      if (i < pieces && xr < M && k < p.K)
-        xv[u] = *reinterpret_cast<const uint4*>(p.x + static_cast<int64_t>(m0 + xr) * p.x_stride + k);
+      if (i < pieces && xr < p.M && k < p.K)
+        xv[u] = *reinterpret_cast<const uint4*>(p.x + static_cast<int64_t>(xr) * p.x_stride + k);
     }
   };
   auto stage_x = [&](int i0) {
 #pragma unroll
     for (int u = 0; u < kBatch; ++u) {
-      const int i = i0 + u * blockDim.x;
+      const int i = i0 + u * kThreads;
       const int xr = (i / 16) % RT, chunk = i / (16 * RT);
       if (i < pieces)
         *reinterpret_cast<uint4*>(xs + (chunk * RT + xr) * kXPitch + 4 * m16) = as_operand(xv[u]);
@@ -211,13 +274,13 @@ __global__ void __launch_bounds__(kThreads, RT <= 16 ? 4 : 2) linear_w4_kernel(W
   };
   load_x(threadIdx.x);
   __builtin_amdgcn_sched_barrier(0);
-  Codes buf[D];
+  typename Stream::Step buf[D];
 #pragma unroll
   for (int d = 0; d < D; ++d)
-    if (mine + d * WK < end) load(mine + d * WK, buf[d]);
+    if (mine + d * WK < end) codes.load(mine + d * WK, buf[d]);
   __builtin_amdgcn_sched_barrier(0);
   stage_x(threadIdx.x);
-  for (int i0 = threadIdx.x + kBatch * blockDim.x; i0 < pieces; i0 += kBatch * blockDim.x) {
+  for (int i0 = threadIdx.x + kBatch * kThreads; i0 < pieces; i0 += kBatch * kThreads) {
     load_x(i0);
     stage_x(i0);
   }
@@ -226,81 +289,53 @@ __global__ void __launch_bounds__(kThreads, RT <= 16 ? 4 : 2) linear_w4_kernel(W
   const int xrow = RT < 16 ? m16 & (RT - 1) : m16;     // an operand row that is not staged repeats one that is
   const bf16x8_t ones = __builtin_bit_cast(bf16x8_t, make_uint4(0x3F803F80u, 0x3F803F80u, 0x3F803F80u, 0x3F803F80u));
   const CodeBits bits;
-  f32x4_t acc[NT][MT];
-#pragma unroll
-  for (int q = 0; q < NT; ++q)
-#pragma unroll
-    for (int m = 0; m < MT; ++m) acc[q][m] = f32x4_t{0.f, 0.f, 0.f, 0.f};
   const f32x4_t none = f32x4_t{0.f, 0.f, 0.f, 0.f};
-  // TU chunks of a step side by side, where registers allow: their chains of
-  // products are independent
-  constexpr int TU = MT == 1 ? 2 : 1;
-  auto compute = [&](int c, const Codes& b) {
+  f32x4_t acc[1][1] = {{none}};
+  auto compute = [&](int c, const typename Stream::Step& b) {
     const uint32_t* step = xs + (c - first) * 2 * RT * kXPitch;
-    uint32_t sz[NT][4 * kLoads];                       // scale (low half) and zero of each group
+    uint32_t sz[4 * kLoads];                           // scale (low half) and zero of each group
 #pragma unroll
-    for (int q = 0; q < NT; ++q)
-#pragma unroll
-      for (int i = 0; i < kLoads; ++i) {
-        uint32_t v[4] = {b.s[q][i] | (b.z[q][i] << 16), 0, 0, 0};
-        if constexpr (kGroups >= 4) {
-          broadcast(v);
-        } else {
-          v[1] = v[0];
-          swap16(v[0], v[1]);
-        }
-#pragma unroll
-        for (int j = 0; j < 4; ++j) sz[q][4 * i + j] = v[j];
+    for (int i = 0; i < kLoads; ++i) {
+      uint32_t v[4] = {b.s[0][i] | (b.z[0][i] << 16), 0, 0, 0};
+      if constexpr (kGroups >= 4) {
+        broadcast(v);
+      } else {
+        v[1] = v[0];
+        swap16(v[0], v[1]);
       }
 #pragma unroll
-    for (int t0 = 0; t0 < 2; t0 += TU) {
-      uint32_t w[NT][TU][4];
+      for (int j = 0; j < 4; ++j) sz[4 * i + j] = v[j];
+    }
+    // the step's two chunks side by side: their chains of products are independent
+    uint32_t w[2][4];
 #pragma unroll
-      for (int q = 0; q < NT; ++q)
+    for (int t = 0; t < 2; ++t) {
+      const uint4 v = b.w[0][t];
+      w[t][0] = v.x; w[t][1] = v.y; w[t][2] = v.z; w[t][3] = v.w;
+      if constexpr (PER < 4) transpose(w[t]);
+    }
+    f32x4_t sum[2], xsum[2];                           // of a group: codes by x, and x
 #pragma unroll
-        for (int t = 0; t < TU; ++t) {
-          const uint4 v = b.w[q][t0 + t];
-          w[q][t][0] = v.x; w[q][t][1] = v.y; w[q][t][2] = v.z; w[q][t][3] = v.w;
-          if constexpr (PER < 4) transpose(w[q][t]);
-        }
-      f32x4_t sum[TU][NT][MT], xsum[TU][MT];           // of a group: codes by x, and x
+    for (int d = 0; d < 4; ++d) {
 #pragma unroll
-      for (int d = 0; d < 4; ++d) {
+      for (int t = 0; t < 2; ++t) {
+        const bf16x8_t xo = *reinterpret_cast<const bf16x8_t*>(
+            step + (t * RT + xrow) * kXPitch + (PER < 4 ? 16 * d + 4 * g : 16 * g + 4 * d));
+        xsum[t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(xo, ones, d % PER == 0 ? none : xsum[t], 0, 0, 0);
+        sum[t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(xo, bits.operand(w[t][d]),
+                                                         d % PER == 0 ? none : sum[t], 0, 0, 0);
+      }
+      if (d % PER == PER - 1) {
 #pragma unroll
-        for (int t = 0; t < TU; ++t) {
-          bf16x8_t wo[NT];
+        for (int t = 0; t < 2; ++t) {
+          const int i = t * (4 / PER) + d / PER;
+          const float s = __uint_as_float(sz[i] << 16), z = 16.0f + static_cast<float>(sz[i] >> 16);
 #pragma unroll
-          for (int q = 0; q < NT; ++q) wo[q] = bits.operand(w[q][t][d]);
-#pragma unroll
-          for (int m = 0; m < MT; ++m) {
-            const bf16x8_t xo = *reinterpret_cast<const bf16x8_t*>(
-                step + ((t0 + t) * RT + 16 * m + xrow) * kXPitch + (PER < 4 ? 16 * d + 4 * g : 16 * g + 4 * d));
-            xsum[t][m] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(xo, ones, d % PER == 0 ? none : xsum[t][m], 0, 0, 0);
-#pragma unroll
-            for (int q = 0; q < NT; ++q)
-              sum[t][q][m] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(
-                  xo, wo[q], d % PER == 0 ? none : sum[t][q][m], 0, 0, 0);
-          }
-        }
-        if (d % PER == PER - 1) {
-#pragma unroll
-          for (int t = 0; t < TU; ++t) {
-            const int i = (t0 + t) * (4 / PER) + d / PER;
-#pragma unroll
-            for (int q = 0; q < NT; ++q) {
-              const float s = __uint_as_float(sz[q][i] << 16), z = 16.0f + static_cast<float>(sz[q][i] >> 16);
-#pragma unroll
-              for (int m = 0; m < MT; ++m) {
-#pragma unroll
-                for (int e = 0; e < 4; ++e)
-                  acc[q][m][e] =
-                      __builtin_fmaf(s, __builtin_fmaf(-z, xsum[t][m][e], sum[t][q][m][e]), acc[q][m][e]);
-                // the sums so far are wanted here: put off to the end of the
-                // step, the operands of all its groups stay in registers and spill
-                asm("" : "+v"(acc[q][m]));
-              }
-            }
-          }
+          for (int e = 0; e < 4; ++e)
+            acc[0][0][e] = __builtin_fmaf(s, __builtin_fmaf(-z, xsum[t][e], sum[t][e]), acc[0][0][e]);
+          // the sums so far are wanted here: put off to the end of the step, the
+          // operands of all its groups stay in registers and spill
+          asm("" : "+v"(acc[0][0]));
         }
       }
     }
@@ -310,51 +345,188 @@ __global__ void __launch_bounds__(kThreads, RT <= 16 ? 4 : 2) linear_w4_kernel(W
     for (int d = 0; d < D; ++d) {
       const int c = c0 + d * WK;
       if (c < end) compute(c, buf[d]);
-      if (c + D * WK < end) load(c + D * WK, buf[d]);
+      if (c + D * WK < end) codes.load(c + D * WK, buf[d]);
     }
   }
+  if constexpr (WK > 1) __syncthreads();
+  store_tiles<1, 1, WK>(p, acc, xs, wv, lane, n0, blockIdx.y, 0, p.M);
+}
 
-  if constexpr (WK > 1) {
-    // the waves of a tile meet in LDS and are summed in wave order (deterministic)
-    __syncthreads();
-    f32x4_t* const sums = reinterpret_cast<f32x4_t*>(xs);
+// A wave's LDS accesses happen in order; this keeps the compiler to it where lanes
+// read what others of their wave have written.
+__device__ __forceinline__ void in_order() {
+  __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+  __builtin_amdgcn_wave_barrier();
+}
+
+// More rows, in slabs of 64 (MT tiles of 16 staged).  A wave holds two tiles of 16
+// weight rows; the 8 / WK waves of the same step share its x, a chunk at a time in
+// LDS (with one wave a step its own), the next one or two chunks in registers.
+// The zeros' part of a sum, -scale (16 + zero) sum x, is a product of its own over
+// four groups (fp32 operands; a scale times an integer up to 31 is exact).
+template <int MT, int PER, int WK>
+__global__ void __launch_bounds__(kThreads, 2) linear_w4_slab_kernel(W4Params p) {
+  constexpr int NT = 2, D = 2;
+  using Stream = CodeStream<PER, NT>;
+  constexpr int kGroups = Stream::kGroups, kLoads = Stream::kLoads;
+  constexpr int kShare = kWaves / WK, kBufs = kShare > 1 ? 2 : 1;
+  constexpr int kPieces = 4 * MT / kShare;             // of a chunk, four rows each, that a wave stages
+  constexpr int kAhead = kPieces >= 8 ? 1 : 2;         // chunks on their way in registers
+  extern __shared__ __attribute__((aligned(16))) uint32_t xs[];
+  const int lane = threadIdx.x & (kWave - 1);
+  const int wv = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
+  const int m16 = lane & 15, g = lane >> 4;
+  const int n0 = 16 * NT * (blockIdx.x * kShare + wv / WK);
+  const int m0 = blockIdx.z * 64;
+  const int M = p.M - m0 < 64 ? p.M - m0 : 64;
+  const int nsteps = (p.K + kStepK - 1) / kStepK;
+  const int first = static_cast<int>(static_cast<int64_t>(nsteps) * blockIdx.y / gridDim.y);
+  const int end = static_cast<int>(static_cast<int64_t>(nsteps) * (blockIdx.y + 1) / gridDim.y);
+  const int mine = first + wv % WK;
+  const int kend = end * kStepK < p.K ? end * kStepK : p.K;
+  const Stream codes(p, n0, lane);
+
+  // x past its last row or the end of the range is zero: outside the descriptor,
+  // which ends with row M - 1 (at most 2^31 bytes: the caller has checked)
+  const uint32_t stride = static_cast<uint32_t>(p.x_stride);
+  const __amdgpu_buffer_rsrc_t xr = make_rsrc(p.x + static_cast<int64_t>(m0) * p.x_stride,
+                                              static_cast<int>(2 * (stride * (M - 1) + p.K)));
+  uint32_t* const stage = xs + (wv % WK) * kBufs * (16 * MT * kXPitch);
+  const int member = wv / WK * kPieces;                // this wave's first piece
+  const uint32_t xlane = stride * 2 * (4 * member + g) + 16 * m16;
+  uint4 xv[kAhead][kPieces];
+  auto load_x = [&](int c, int t) {
+    const int k = c * kStepK + kChunkK * t;
+    const uint32_t at = k + 8 * m16 < kend ? xlane + 2 * k : 0x80000000u;
 #pragma unroll
-    for (int q = 0; q < NT; ++q)
+    for (int u = 0; u < kPieces; ++u)
+      xv[t % kAhead][u] = __builtin_bit_cast(
+          uint4, __builtin_amdgcn_raw_buffer_load_b128(xr, static_cast<int>(at + stride * (8 * u)), 0, 0));
+  };
+  auto stage_x = [&](int t) {
 #pragma unroll
-      for (int m = 0; m < MT; ++m) sums[((wv * NT + q) * MT + m) * kWave + lane] = acc[q][m];
-    __syncthreads();
+    for (int u = 0; u < kPieces; ++u)
+      *reinterpret_cast<uint4*>(stage + (t % kBufs * 16 * MT + 4 * (member + u) + g) * kXPitch + 4 * m16) =
+          as_operand(xv[t % kAhead][u]);
+  };
+#pragma unroll
+  for (int t = 0; t < kAhead; ++t) load_x(mine, t);
+  __builtin_amdgcn_sched_barrier(0);
+  typename Stream::Step buf[D];
+#pragma unroll
+  for (int d = 0; d < D; ++d)
+    if (mine + d * WK < end) codes.load(mine + d * WK, buf[d]);
+  __builtin_amdgcn_sched_barrier(0);
+
+  // operand rows 4 d .. 4 d + 3 of ones: the product with x leaves the sum of x's
+  // row l % 16 in lane quarter d, as the fp32 product takes it
+  bf16x8_t ones[4];
+#pragma unroll
+  for (int d = 0; d < 4; ++d) {
+    const uint32_t v = m16 / 4 == d ? 0x3F803F80u : 0u;
+    ones[d] = __builtin_bit_cast(bf16x8_t, make_uint4(v, v, v, v));
   }
-
-  // a lane's column n of four rows; the tiles of 16 x 16 are dealt to the waves
-  // that share them
+  const CodeBits bits;
+  const f32x4_t none = f32x4_t{0.f, 0.f, 0.f, 0.f};
+  f32x4_t acc[NT][MT];
 #pragma unroll
-  for (int qm = 0; qm < NT * MT; ++qm) {
-    const int q = qm / MT, m = qm % MT;
-    f32x4_t sum = acc[q][m];
-    if constexpr (WK > 1) {
-      if (qm % WK != wv % WK) continue;
-      const f32x4_t* at = reinterpret_cast<const f32x4_t*>(xs) + ((wv / WK * WK) * NT * MT + qm) * kWave + lane;
-      sum = at[0];
+  for (int q = 0; q < NT; ++q)
 #pragma unroll
-      for (int v = 1; v < WK; ++v) {
-        const f32x4_t a = at[v * NT * MT * kWave];
+    for (int m = 0; m < MT; ++m) acc[q][m] = none;
+  auto compute = [&](int c, const typename Stream::Step& b) {
+    uint32_t scale[NT][4];                             // of group d and, in the high half, 4 + d
+    float below[NT][kLoads];                           // -scale (16 + zero) of the lane quarter's groups
 #pragma unroll
-        for (int e = 0; e < 4; ++e) sum[e] += a[e];
+    for (int q = 0; q < NT; ++q) {
+      scale[q][0] = kLoads == 2 ? b.s[q][0] | b.s[q][kLoads - 1] << 16 : b.s[q][0];
+#pragma unroll
+      for (int i = 0; i < kLoads; ++i)
+        below[q][i] = -__uint_as_float(b.s[q][i] << 16) * (16.0f + static_cast<float>(b.z[q][i]));
+      if constexpr (kGroups >= 4) {
+        broadcast(scale[q]);
+      } else {
+        scale[q][1] = scale[q][0];
+        swap16(scale[q][0], scale[q][1]);
       }
     }
-    const int n = n0 + 16 * q + m16;
-    if (n >= p.N) continue;
-    const float bias = !p.partial && p.bias ? bf16_to_f32(p.bias[n]) : 0.0f;
+    f32x4_t sum[NT][MT], xsum[MT];
 #pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      const int r = 16 * m + 4 * g + e;
-      if (r >= M) continue;
-      if (p.partial)
-        p.partial[(static_cast<int64_t>(split) * p.M + m0 + r) * p.N + n] = sum[e];
+    for (int t = 0; t < 2; ++t) {
+      uint32_t w[NT][4];
+#pragma unroll
+      for (int q = 0; q < NT; ++q) {
+        const uint4 v = b.w[q][t];
+        w[q][0] = v.x; w[q][1] = v.y; w[q][2] = v.z; w[q][3] = v.w;
+        if constexpr (PER < 4) transpose(w[q]);
+      }
+      if constexpr (kShare == 1) in_order();
+      stage_x(t);
+      if constexpr (kShare == 1) in_order();
+      if (kAhead == 2)
+        load_x(c + WK, t);
+      else if (t == 0)
+        load_x(c, 1);
       else
-        p.out[static_cast<int64_t>(m0 + r) * p.out_stride + n] = f32_to_bf16(sum[e] + bias);
+        load_x(c + WK, 0);
+      // two buffers: whoever writes one again has passed the barrier behind the
+      // other's use of it
+      if constexpr (kShare > 1) __syncthreads();
+#pragma unroll
+      for (int d = 0; d < 4; ++d) {
+        constexpr int kJoined = 4 * PER < 8 ? 4 * PER : 8;   // products whose sums of x are joined: four groups, or the step
+        const int j = 4 * t + d, group = j / PER;
+        bf16x8_t wo[NT];
+#pragma unroll
+        for (int q = 0; q < NT; ++q) wo[q] = bits.operand(w[q][d]);
+#pragma unroll
+        for (int m = 0; m < MT; ++m) {
+          const bf16x8_t xo = *reinterpret_cast<const bf16x8_t*>(
+              stage + (t % kBufs * 16 * MT + 16 * m + m16) * kXPitch + (PER < 4 ? 16 * d + 4 * g : 16 * g + 4 * d));
+          xsum[m] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(ones[group % 4], xo,
+                                                            j % kJoined == 0 ? none : xsum[m], 0, 0, 0);
+#pragma unroll
+          for (int q = 0; q < NT; ++q)
+            sum[q][m] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(xo, wo[q], j % PER == 0 ? none : sum[q][m], 0, 0, 0);
+        }
+        if (j % PER == PER - 1) {
+#pragma unroll
+          for (int q = 0; q < NT; ++q) {
+            const uint32_t two = scale[q][group % 4];
+            const float s = __uint_as_float(group / 4 ? two & 0xFFFF0000u : two << 16);
+#pragma unroll
+            for (int m = 0; m < MT; ++m) {
+#pragma unroll
+              for (int e = 0; e < 4; ++e) acc[q][m][e] = __builtin_fmaf(s, sum[q][m][e], acc[q][m][e]);
+              asm("" : "+v"(acc[q][m]));               // not put off, as above
+            }
+          }
+        }
+        if (j % kJoined == kJoined - 1) {
+#pragma unroll
+          for (int q = 0; q < NT; ++q)
+#pragma unroll
+            for (int m = 0; m < MT; ++m)
+              acc[q][m] = __builtin_amdgcn_mfma_f32_16x16x4f32(xsum[m][0], below[q][group / 4], acc[q][m], 0, 0, 0);
+        }
+      }
+    }
+  };
+  // waves that share a barrier go as many rounds as the first of them
+  for (int c0 = mine; c0 - mine + first < end; c0 += D * WK) {
+#pragma unroll
+    for (int d = 0; d < D; ++d) {
+      const int c = c0 + d * WK;
+      if (c < end) {
+        compute(c, buf[d]);
+      } else if (kShare > 1 && c - mine + first < end) {
+        __syncthreads();
+        __syncthreads();
+      }
+      if (c + D * WK < end) codes.load(c + D * WK, buf[d]);
     }
   }
+  if constexpr (WK > 1) __syncthreads();
+  store_tiles<NT, MT, WK>(p, acc, xs, wv, lane, n0, blockIdx.y, m0, M);
 }
 
 // The sum of the K ranges' parts, in order: a thread owns V columns of a row and
@@ -384,46 +556,60 @@ __global__ void __launch_bounds__(256) linear_w4_sum_kernel(W4Params p, int32_t 
   for (int e = 0; e < V; ++e) o[e] = f32_to_bf16(p.bias ? s[e] + bf16_to_f32(p.bias[n + e]) : s[e]);
 }
 
-// Rows of x a workgroup stages, ranges of K, waves of a workgroup, and how many of
-// them share a tile of weight rows.
+// Rows of x a workgroup stages, ranges of K, and waves that share a tile of weight
+// rows.
 struct W4Plan {
-  int32_t rows, splits, waves, shared;
+  int32_t rows, splits, shared;
 };
 
-// Tiles of 16 weight rows a wave holds with RT rows of x.
-constexpr int tiles_of(int rt) { return rt <= 16 ? 1 : 2; }
+// LDS of a workgroup: its range's x (up to 16 rows; more: a chunk or two for every
+// step under way), and room for the waves' tiles behind.
+int lds_bytes(const W4Plan& plan, int32_t k) {
+  const int steps = ((k + kStepK - 1) / kStepK + plan.splits - 1) / plan.splits;
+  const bool slab = plan.rows > 16;
+  const int staged = !slab ? 2 * steps : plan.shared == kWaves ? kWaves : 2 * plan.shared;
+  const int x = staged * plan.rows * kXPitch * 4;
+  const int tiles = plan.shared > 1 ? kThreads * (slab ? 2 * (plan.rows / 16) : 1) * 16 : 0;
+  return x > tiles ? x : tiles;
+}
 
-template <int RT, int PER, int NT, int D, int WK>
+// More than the default bound of dynamic LDS, once per device and kernel.
+template <void (*Kernel)(W4Params)>
+bool allow_lds() {
+  static bool set[64] = {};
+  int dev = 0;
+  if (hipGetDevice(&dev) != hipSuccess) return false;
+  const bool known = dev >= 0 && dev < 64;
+  if (known && set[dev]) return true;
+  if (hipFuncSetAttribute(reinterpret_cast<const void*>(Kernel), hipFuncAttributeMaxDynamicSharedMemorySize,
+                          kMaxLds) != hipSuccess)
+    return false;
+  if (known) set[dev] = true;
+  return true;
+}
+
+template <int RT, int PER, int WK>
 int launch(const W4Params& p, const W4Plan& plan, hipStream_t s) {
-  const int steps = ((p.K + kStepK - 1) / kStepK + plan.splits - 1) / plan.splits;
-  int bytes = steps * 2 * RT * kXPitch * 4;
-  const int sums = plan.waves * kWave * NT * (RT <= 16 ? 1 : RT / 16) * 16;
-  if (WK > 1 && bytes < sums) bytes = sums;
-  const int tile = 16 * NT * (plan.waves / WK);
-  const dim3 grid((p.N + tile - 1) / tile, plan.splits, (p.M + 63) / 64);
-  auto* kern = linear_w4_kernel<RT, PER, NT, D, WK>;
-  if (bytes > 64 * 1024) {
-    // more than the default bound of dynamic LDS, once per device
-    static bool set[64] = {};
-    int dev = 0;
-    if (hipGetDevice(&dev) != hipSuccess) return NVA_ERR_LAUNCH;
-    if (dev < 0 || dev >= 64 || !set[dev]) {
-      if (hipFuncSetAttribute(reinterpret_cast<const void*>(kern),
-                              hipFuncAttributeMaxDynamicSharedMemorySize, kMaxLds) != hipSuccess)
-        return NVA_ERR_LAUNCH;
-      if (dev >= 0 && dev < 64) set[dev] = true;
-    }
+  const int bytes = lds_bytes(plan, p.K);
+  if constexpr (RT > 16) {
+    constexpr auto kern = linear_w4_slab_kernel<RT / 16, PER, WK>;
+    if (bytes > 64 * 1024 && !allow_lds<kern>()) return NVA_ERR_LAUNCH;
+    const int tile = 32 * (kWaves / WK);
+    kern<<<dim3((p.N + tile - 1) / tile, plan.splits, (p.M + 63) / 64), kThreads, bytes, s>>>(p);
+  } else {
+    constexpr auto kern = linear_w4_kernel<RT, PER, WK>;
+    if (bytes > 64 * 1024 && !allow_lds<kern>()) return NVA_ERR_LAUNCH;
+    const int tile = 16 * (kWaves / WK);
+    kern<<<dim3((p.N + tile - 1) / tile, plan.splits), kThreads, bytes, s>>>(p);
   }
-  kern<<<grid, plan.waves * kWave, bytes, s>>>(p);
   return launch_status();
 }
 
 template <int RT, int WK>
 int launch_rows(const W4Params& p, const W4Plan& plan, hipStream_t s) {
-  constexpr int NT = tiles_of(RT), D = 3;
-  if (p.per_group % 4 == 0) return launch<RT, 4, NT, D, WK>(p, plan, s);
-  if (p.per_group % 2 == 0) return launch<RT, 2, NT, D, WK>(p, plan, s);
-  return launch<RT, 1, NT, D, WK>(p, plan, s);
+  if (p.per_group % 4 == 0) return launch<RT, 4, WK>(p, plan, s);
+  if (p.per_group % 2 == 0) return launch<RT, 2, WK>(p, plan, s);
+  return launch<RT, 1, WK>(p, plan, s);
 }
 
 template <int RT>
@@ -450,46 +636,55 @@ int32_t device_cus() {
 }
 
 // The ranges of K and the waves that share a tile, by the least modelled time
-// (us): rounds of workgroups over the device, each a wave's steps (longer with
-// more waves a SIMD, shorter groups and more rows) and the staging of its x, and
-// with several ranges the summing kernel.  The constants are a fit to 18 shapes
-// (1-64 rows, N 800-151936, K 640-25600, groups of 32-128) timed over all
-// choices: its choice is 3% from the best on the geometric mean.
+// (us): rounds of workgroups over the device, each a wave's steps and what comes
+// before and behind them, and with several ranges the summing kernel.
+//   * Up to 16 rows two workgroups share a CU and its time; a range's x is staged
+//     first, and LDS bounds the range.  Fitted to 18 shapes (1-64 rows, N 800-151936,
+//     K 640-25600, groups of 32-128) timed over all choices, where its choice is 3%
+//     from the best: 1 x 4096 x 4096 one range with eight waves a tile 5.5 us, with
+//     four 7.2, eight ranges with one 7.4; 16 x 5120 x 25600 twelve ranges 23.9, six
+//     24.3, sixteen 25.3.
+//   * More rows take a CU a workgroup; a step costs more where fewer waves share its
+//     x.  Fitted to 17 shapes (17-256 rows, N 1024-151936, K 512-25600), 1% from the
+//     best: 61 x 6144 x 4096 one range with eight waves a tile 17.7 us, two with four
+//     19.8, eight with one 24.9; 64 x 24576 x 4096 one with two 37, with eight 43.
 W4Plan make_plan(int32_t rows, int32_t n, int32_t k, int32_t group) {
-  W4Plan best = {};
-  best.rows = rows <= 4 ? 4 : rows <= 8 ? 8 : rows <= 16 ? 16 : rows <= 32 ? 32 : 64;
-  best.waves = kWaves;
-  const int rt = best.rows, nt = tiles_of(rt), mt = rt <= 16 ? 1 : rt / 16;
-  const int per = group % 128 == 0 ? 4 : group % 64 == 0 ? 2 : 1;
-  const int step_bytes = 2 * rt * kXPitch * 4;
-  const int32_t steps = (k + kStepK - 1) / kStepK, most = kMaxLds / step_bytes;
+  W4Plan best = {}, plan = {};
+  plan.rows = rows <= 4 ? 4 : rows <= 8 ? 8 : rows <= 16 ? 16 : rows <= 32 ? 32 : 64;
+  const bool slab = plan.rows > 16;
+  const int rt = plan.rows;
+  const int parts = group % 128 == 0 ? 1 : group % 64 == 0 ? 2 : 4;   // groups of a chunk, if they end in it
+  const int32_t steps = (k + kStepK - 1) / kStepK, most = slab ? steps : kMaxLds / (2 * rt * kXPitch * 4);
+  const int32_t fewest = (steps + most - 1) / most;
   const int64_t cus = device_cus(), slabs = (rows + 63) / 64;
-  const float unit = 0.53f * nt * (1.0f + 0.22f * (mt - 1)) * (1.0f + 0.23f * (4 / per - 1));
-  const int slots = rt <= 16 ? 2 : 1;                  // workgroups of a CU by registers
   float least = 0.0f;
   for (int shared = 1; shared <= kWaves; shared *= 2) {
-    const int tile = 16 * nt * (kWaves / shared);
+    const int tile = (slab ? 32 : 16) * (kWaves / shared);
     const int64_t tiles = (n + tile - 1) / tile * slabs;
-    const int32_t fewest = (steps + most - 1) / most;
     for (int fill = 0; fill <= 4; fill = fill ? 2 * fill : 1) {
       // as few ranges as LDS allows, or as many as make one, two, four rounds
-      int32_t splits = fill ? static_cast<int32_t>(fill * cus / tiles) : fewest;
+      const int32_t splits = fill ? static_cast<int32_t>(fill * cus / tiles) : fewest;
       if (splits < fewest || (fill && splits == fewest) || splits > steps) continue;
+      plan.splits = splits;
+      plan.shared = shared;
       const int32_t of_range = (steps + splits - 1) / splits;
-      int bytes = of_range * step_bytes;
-      const int parked = kThreads * nt * mt * 16;
-      if (shared > 1 && bytes < parked) bytes = parked;
-      const int fit = kMaxLds / bytes < slots ? kMaxLds / bytes : slots;
+      const int32_t of_wave = (of_range + shared - 1) / shared;
       const int64_t per_cu = (tiles * splits + cus - 1) / cus;
-      const int64_t at_once = per_cu < fit ? per_cu : fit;
-      float t = unit * ((of_range + shared - 1) / shared) * (at_once > 1 ? at_once : 1.0f) +
-                0.014f * of_range * rt + (shared > 1 ? 0.012f * nt * mt * shared : 0.0f);
-      t *= static_cast<float>((per_cu + at_once - 1) / at_once);
-      if (splits > 1) t += 2.3f + 2.8e-6f * splits * rows * n;
+      float t;
+      if (slab) {
+        const float step = (rt == 64 ? 2.15f : 1.53f) * (1.0f + 0.065f * (parts - 1)) * (1.0f + 0.04f * shared);
+        t = (step * of_wave + 1.3f) * per_cu;
+        if (splits > 1) t += 2.8f + 1.9e-6f * splits * rows * n;
+      } else {
+        const int64_t fit = 2 * lds_bytes(plan, k) <= kMaxLds && per_cu > 1 ? 2 : 1;
+        t = 0.53f * (1.0f + 0.23f * (parts - 1)) * of_wave * fit + 0.014f * of_range * rt;
+        if (shared > 1) t += 0.012f * shared;
+        t *= static_cast<float>((per_cu + fit - 1) / fit);
+        if (splits > 1) t += 2.3f + 2.8e-6f * splits * rows * n;
+      }
       if (best.splits == 0 || t < least) {
         least = t;
-        best.splits = splits;
-        best.shared = shared;
+        best = plan;
       }
     }
   }
@@ -523,6 +718,8 @@ extern "C" int nva_linear_w4(const void* x, int64_t x_row_stride, const void* qw
   if (group % 32 || x_row_stride % 8 || !aligned16(x) || !aligned16(qweight) || rows > 64 * 65535 ||
       k > (1 << 20) || static_cast<int64_t>(k / group) * n >= 1 << 29)
     return NVA_ERR_UNSUPPORTED;
+  // a slab of x is addressed in 31 bits
+  if (rows > 16 && (rows < 64 ? rows : 64) * x_row_stride >= 1 << 30) return NVA_ERR_UNSUPPORTED;
   const W4Plan plan = make_plan(rows, n, k, group);
   const size_t need = plan_bytes(plan, rows, n);
   if (need && (!workspace || workspace_bytes < need || !aligned16(workspace))) return NVA_ERR_WORKSPACE;

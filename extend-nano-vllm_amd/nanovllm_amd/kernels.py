@@ -874,8 +874,9 @@ def linear_w4(x: torch.Tensor, qweight: torch.Tensor, scales: torch.Tensor,
     G = k / scales.shape[0], in float32, rounded to bf16 once (no weight is
     rounded).  x: bf16 [rows, k]; qweight: uint8 [n, k / 2], element 2 i in the
     low half of byte i; scales: bf16 [k / G, n]; zeros: uint8 [k / G, n] of 0..15,
-    None for 8; bias: bf16 [n].  G is a multiple of 32.  Made for up to 64 rows
-    (a step's tokens); more rows run 64 at a time.  A row of x that holds an
+    None for 8; bias: bf16 [n].  G is a multiple of 32; k <= 2^20, k n / G < 2^29.
+    Made for up to 64 rows (a step's tokens); more rows run 64 at a time.  out must
+    not overlap the inputs.  A row of x that holds an
     infinity or a NaN comes out NaN."""
     got = (_front or _front_end()).linear_w4(x, qweight, scales, zeros, bias, out)
     if got is not None:
@@ -907,9 +908,9 @@ def linear_w4(x: torch.Tensor, qweight: torch.Tensor, scales: torch.Tensor,
         raise ValueError("out must be bf16 [rows, n] with unit last stride")
     if n == 0 or rows == 0:
         return out
-    # the kernel reads x 16 bytes at a time
+    # the kernel reads x 16 bytes at a time, and 64 rows of it within 2^31 bytes
     if x.stride(1) != 1 or (rows > 1 and (x.stride(0) % 8 or x.stride(0) < k)) \
-            or x.data_ptr() % 16:
+            or (rows > 16 and min(rows, 64) * x.stride(0) >= 1 << 30) or x.data_ptr() % 16:
         x = x.clone(memory_format=torch.contiguous_format)
     if rows > 1 and out.stride(0) < n:
         raise ValueError("out rows must not overlap")

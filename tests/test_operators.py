@@ -143,7 +143,10 @@ def test_the_library_refuses_bad_products_on_the_host():
     for kw in (dict(rows=-1), dict(n=0), dict(k=0), dict(group=0), dict(group=48), dict(x=None),
                dict(w=None), dict(s=None), dict(out=None), dict(stride=120), dict(out_stride=7)):
         assert call(**kw) == _native.NVA_ERR_ARG, kw
-    for kw in (dict(group=16), dict(stride=132), dict(x=P + 8), dict(w=P + 4)):
+    for kw in (dict(group=16), dict(stride=132), dict(x=P + 8), dict(w=P + 4),
+               dict(rows=64, stride=1 << 24), dict(rows=17, stride=1 << 26),
+               dict(rows=64 * 65535 + 1), dict(k=(1 << 20) + 32, stride=1 << 21),
+               dict(n=1 << 27, out_stride=1 << 27)):
         assert call(**kw) == _native.NVA_ERR_UNSUPPORTED, kw
 
 

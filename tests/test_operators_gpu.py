@@ -75,7 +75,10 @@ def w4_reference(x, qw, s, z, b):
     (5, 18, 192, 64), (8, 130, 256, 128), (15, 64, 1024, 128), (16, 255, 544, 32),
     (17, 48, 384, 64), (31, 20, 1152, 128), (32, 512, 2048, 256), (33, 96, 640, 32),
     (61, 77, 1280, 64), (64, 260, 4096, 128), (65, 34, 320, 32), (130, 50, 768, 384),
-    (1, 4096, 4096, 128), (6, 1030, 4160, 64), (16, 2048, 2560, 32), (1, 40, 96, 96)])
+    (1, 4096, 4096, 128), (6, 1030, 4160, 64), (16, 2048, 2560, 32), (1, 40, 96, 96),
+    (17, 5000, 544, 32), (20, 9000, 288, 96), (24, 2500, 1088, 64), (40, 1100, 6400, 256),
+    (48, 16400, 512, 128), (64, 8200, 1056, 32), (64, 600, 9728, 128), (81, 4000, 2080, 32),
+    (130, 700, 4416, 64), (257, 130, 2048, 128)])
 @pytest.mark.parametrize("zeros,bias", [(False, False), (True, True)])
 def test_linear_w4(cuda, rows, n, k, group, zeros, bias):
     case = w4_case(rows, n, k, group, zeros, bias, seed=rows + n)
@@ -98,6 +101,30 @@ def test_linear_w4_strides_out_and_alignment(cuda):
     assert got.data_ptr() == out[:, 2:].data_ptr()
     close(out[:, 2:38], want, tol)
     assert (out[:, :2] == 7).all() and (out[:, 38:] == 7).all()
+
+
+def test_linear_w4_rows_far_apart(cuda):
+    """Rows whose 64 together pass 2^31 bytes (a column of a wide tensor)."""
+    x, qw, s, z, b = w4_case(33, 36, 256, 64, True, True)
+    want, tol = w4_reference(x, qw, s, z, b)
+    for stride in ((1 << 30) // 33 // 8 * 8, (1 << 30) // 33 // 8 * 8 + 8):
+        flat = torch.empty(32 * stride + 256, dtype=BF16, device="cuda")
+        far = flat.as_strided((33, 256), (stride, 1))
+        far.copy_(x)
+        close(K.linear_w4(far, qw, s, z, b), want, tol)
+        del flat, far
+
+
+def test_linear_w4_a_bad_row_stays_alone_in_a_slab(cuda):
+    for rows, n in ((29, 4100), (70, 70)):
+        x, qw, s, z, b = w4_case(rows, n, 512, 64, True, False)
+        want, tol = w4_reference(x, qw, s, z, b)
+        bad = torch.zeros(rows, dtype=torch.bool, device="cuda")
+        bad[::9] = True
+        x[::9, 7::100], x[::18, 300] = float("inf"), float("nan")
+        got = K.linear_w4(x, qw, s, z, b)
+        assert got[bad].isnan().all()
+        close(got[~bad], want[~bad], tol[~bad])
 
 
 def test_linear_w4_a_bad_row_stays_alone(cuda):
