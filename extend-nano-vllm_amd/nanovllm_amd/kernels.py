@@ -565,7 +565,9 @@ def shared_prefix_attention_varlen(q: torch.Tensor, k_cache: torch.Tensor, v_cac
     keys must be those that row 0 of ``block_table`` lists: the same pages (the
     prefix cache shares whole ones), or copies of them.  Row 0 lists the whole
     prefix whatever sequence 0's length; a shorter sequence sees its own length
-    of it.  Rows of no sequence are left as they are."""
+    of it.  Rows of no sequence are left as they are.  While the prefix's bytes,
+    counted once a sequence, stay below about 128 MiB (32 MiB in FP8), the paged
+    attention is the faster call."""
     got = (_front or _front_end()).shared_prefix_attention_varlen(
         q, k_cache, v_cache, cu_seqlens_q, cu_seqlens_k, max_seqlen_q, max_seqlen_k, prefix_len,
         softmax_scale, block_table, k_scale, v_scale, out)

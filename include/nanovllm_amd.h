@@ -536,6 +536,8 @@ int nva_rotary_embedding(const int64_t *positions, const double *inv_freq, float
  *   through each sequence's own row.  Everything else as for K1: strides,
  *   dtypes, scales, the clip by max_seqlen_q / max_seqlen_k (which count the
  *   prefix), block ids outside the cache.  Rows of no sequence are not written.
+ *   While the prefix's bytes, counted once a sequence, stay below about 128 MiB
+ *   (32 MiB in FP8), nva_paged_attention_* is the faster call.
  * workspace: nva_shared_prefix_workspace_size(...) bytes, 16-byte aligned, no
  *   initialisation; sized for the call's own shape.
  * ------------------------------------------------------------------- */
