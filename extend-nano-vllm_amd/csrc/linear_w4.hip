@@ -718,8 +718,9 @@ extern "C" int nva_linear_w4(const void* x, int64_t x_row_stride, const void* qw
   if (group % 32 || x_row_stride % 8 || !aligned16(x) || !aligned16(qweight) || rows > 64 * 65535 ||
       k > (1 << 20) || static_cast<int64_t>(k / group) * n >= 1 << 29)
     return NVA_ERR_UNSUPPORTED;
-  // a slab of x is addressed in 31 bits
-  if (rows > 16 && (rows < 64 ? rows : 64) * x_row_stride >= 1 << 30) return NVA_ERR_UNSUPPORTED;
+  // a slab of x is addressed in 31 bits, and what lies 2^31 bytes behind its rows
+  // must not come round to it
+  if (rows > 16 && x_row_stride >= 1 << 24) return NVA_ERR_UNSUPPORTED;
   const W4Plan plan = make_plan(rows, n, k, group);
   const size_t need = plan_bytes(plan, rows, n);
   if (need && (!workspace || workspace_bytes < need || !aligned16(workspace))) return NVA_ERR_WORKSPACE;

@@ -910,9 +910,9 @@ def linear_w4(x: torch.Tensor, qweight: torch.Tensor, scales: torch.Tensor,
         raise ValueError("out must be bf16 [rows, n] with unit last stride")
     if n == 0 or rows == 0:
         return out
-    # the kernel reads x 16 bytes at a time, and 64 rows of it within 2^31 bytes
+    # the kernel reads x 16 bytes at a time, and rows of a slab within 2^31 bytes
     if x.stride(1) != 1 or (rows > 1 and (x.stride(0) % 8 or x.stride(0) < k)) \
-            or (rows > 16 and min(rows, 64) * x.stride(0) >= 1 << 30) or x.data_ptr() % 16:
+            or (rows > 16 and x.stride(0) >= 1 << 24) or x.data_ptr() % 16:
         x = x.clone(memory_format=torch.contiguous_format)
     if rows > 1 and out.stride(0) < n:
         raise ValueError("out rows must not overlap")

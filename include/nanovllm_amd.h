@@ -488,7 +488,7 @@ int nva_linear(const void *x, int64_t x_row_stride, const void *w, void *out,
  *   16-byte aligned (x_row_stride a multiple of 8; NVA_ERR_UNSUPPORTED
  *   otherwise).  Up to 64 * 65535 rows: 64 at a time read the weights once.
  *   Offsets are 32 bits wide: k <= 2^20, k n / group < 2^29, and with more than
- *   16 rows min(rows, 64) * x_row_stride < 2^30 (NVA_ERR_UNSUPPORTED otherwise).
+ *   16 rows x_row_stride < 2^24 (NVA_ERR_UNSUPPORTED otherwise).
  *   out must not overlap the inputs.
  * workspace: nva_linear_w4_workspace_size(rows, n, k, group) bytes (0: none),
  *   16-byte aligned, no initialisation: the parts of ranges of k.

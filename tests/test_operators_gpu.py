@@ -103,13 +103,15 @@ def test_linear_w4_strides_out_and_alignment(cuda):
     assert (out[:, :2] == 7).all() and (out[:, 38:] == 7).all()
 
 
-def test_linear_w4_rows_far_apart(cuda):
-    """Rows whose 64 together pass 2^31 bytes (a column of a wide tensor)."""
-    x, qw, s, z, b = w4_case(33, 36, 256, 64, True, True)
+@pytest.mark.parametrize("rows,k", [(33, 288), (64, 256), (17, 5440)])
+def test_linear_w4_rows_far_apart(cuda, rows, k):
+    """Columns of a wide tensor up to the largest stride that the kernel takes
+    and past it, NaN around them: nothing beside a row comes into its sum."""
+    x, qw, s, z, b = w4_case(rows, 36, k, 32, True, True)
     want, tol = w4_reference(x, qw, s, z, b)
-    for stride in ((1 << 30) // 33 // 8 * 8, (1 << 30) // 33 // 8 * 8 + 8):
-        flat = torch.empty(32 * stride + 256, dtype=BF16, device="cuda")
-        far = flat.as_strided((33, 256), (stride, 1))
+    for stride in ((1 << 24) - 8, 1 << 24):
+        flat = torch.full((rows * stride,), float("nan"), dtype=BF16, device="cuda")
+        far = flat.view(rows, stride)[:, 128:128 + k]
         far.copy_(x)
         close(K.linear_w4(far, qw, s, z, b), want, tol)
         del flat, far
