@@ -659,15 +659,23 @@ PyObject* rotary_embedding(PyObject*, PyObject* const* v, Py_ssize_t n) {
       if (has_k) k_out = k;
     }
     void* s = current_stream(a.device);
+    int status;
     launch([&] {
-      return nva_rotary_embedding(
+      status = nva_rotary_embedding(
           static_cast<const int64_t*>(pos.data_ptr()), static_cast<const double*>(freq.data_ptr()),
           factor, interleaved, dtype, q.data_ptr(), q.stride(0), q.stride(1), hq,
           has_k ? k.data_ptr() : nullptr, has_k ? k.stride(0) : 0, has_k ? k.stride(1) : 0,
           has_k ? hk : 0, t, d, as_i32(2 * freq.size(0)), q_out.data_ptr(), q_out.stride(0),
           q_out.stride(1), has_k ? k_out.data_ptr() : nullptr, has_k ? k_out.stride(0) : 0,
           has_k ? k_out.stride(1) : 0, s);
+      // an error behind the launch (it may be an earlier call's) is not the general
+      // path's to report: what is rotated in place must not be rotated again
+      return status == NVA_ERR_LAUNCH ? NVA_OK : status;
     });
+    if (status != NVA_OK) {
+      PyErr_Format(PyExc_RuntimeError, "rotary_embedding: %s (status %d)", nva_status_string(status), status);
+      return nullptr;
+    }
     PyObject* first = THPVariable_Wrap(q_out);
     PyObject* second = has_k ? THPVariable_Wrap(k_out) : Py_NewRef(Py_None);
     PyObject* both = PyTuple_Pack(2, first, second);

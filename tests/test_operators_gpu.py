@@ -7,7 +7,10 @@ Tolerances.  A rounding to bf16 is off by at most U = 2^-8 of the value, to fp16
 * linear_w4: products of exact operands summed in fp32.  An element's terms are
   (16 + c) x and (16 + z) x, at most 31 |x| each, scaled by s; it passes at most
   32 sums in an MFMA, 4 in a group, 2 in the correction, K / G over the groups
-  and 8 over the waves: (48 + K / G) 2^-24 62 sum |x| s, then U |y|.
+  and 8 over the waves: (48 + K / G) 2^-24 62 sum |x| s, then U |y|.  Where the
+  zeros' part is a product of its own, the K / G sums over the groups come twice
+  but hold one of the two terms more than the other for at most four groups: what
+  they round is at most 31 |x| s in all, and the bound is the same.
 * rotary: sine and cosine are off by at most 2^-22 (truncation 3e-8 and a few
   roundings below one), the products and sums by three roundings:
   2^-21 factor (|x| + |y|), then the type's own rounding.
@@ -15,6 +18,7 @@ Tolerances.  A rounding to bf16 is off by at most U = 2^-8 of the value, to fp16
   exponential are off by less than 2e-4 of it (128 products of operands of
   about one, exp2 to a few ulps): (U + 2e-4) sum p |v| / l, then U |o|.
 """
+import ctypes
 import math
 import random
 
@@ -203,6 +207,27 @@ def rotary_reference(x, positions, freq, interleaved, factor):
         # rounding there is off by up to 2^-25 whatever the value
         rounding = torch.where(tol > 0, rounding.clamp(min=2.0 ** -25), 0.0)
     return y, 2.0 ** -21 * tol + rounding
+
+
+def test_rotary_in_place_turns_once_where_an_earlier_error_is_reported(cuda):
+    """An error that another call has left (here a device number that does not
+    exist) is reported by the launch that follows it; q and k are rotated all the
+    same, and only once."""
+    hip = next(line.split()[-1] for line in open("/proc/self/maps") if "libamdhip64" in line)
+    hip = ctypes.CDLL(hip)
+    q = torch.randn(3, 4, 64, generator=gen(5), device="cuda")
+    k = torch.randn(3, 2, 64, generator=gen(6), device="cuda")
+    pos = torch.tensor([1, 5, 9], device="cuda")
+    freq = torch.rand(32, generator=gen(7), device="cuda", dtype=torch.float64)
+    want = K.rotary_embedding(pos, q, k, freq)
+    rows = torch.cat([q, k], 1)
+    qi, ki = rows[:, :4], rows[:, 4:]
+    torch.cuda.synchronize()
+    assert hip.hipSetDevice(1 << 20) != 0
+    with pytest.raises(RuntimeError):
+        K.rotary_embedding(pos, qi, ki, freq, q_out=qi, k_out=ki)
+    assert torch.equal(qi, want[0]) and torch.equal(ki, want[1])
+    K.rotary_embedding(pos, q, k, freq)      # nothing stays behind
 
 
 @pytest.mark.parametrize("interleaved", [False, True])
