@@ -529,31 +529,27 @@ __global__ void __launch_bounds__(kThreads, 2) linear_w4_slab_kernel(W4Params p)
   store_tiles<NT, MT, WK>(p, acc, xs, wv, lane, n0, blockIdx.y, m0, M);
 }
 
-// The sum of the K ranges' parts, in order: a thread owns V columns of a row and
-// loads kSumBatch parts at a time (one latency, not one a part).
-constexpr int kSumBatch = 8;
-template <int V>
+// The sum of the K ranges' parts, in order.  Bound by latency: a thread loads
+// kSumBatch parts at a time and owns one column, which takes the most workgroups
+// (twelve parts of 1 x 5120: with the main kernel 20.7 us; four columns a thread in
+// batches of eight 21.9).
+constexpr int kSumBatch = 16;
 __global__ void __launch_bounds__(256) linear_w4_sum_kernel(W4Params p, int32_t splits) {
-  typedef __attribute__((ext_vector_type(V))) float vec;
   const int64_t i = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x;
-  const int64_t size = static_cast<int64_t>(p.M) * p.N / V;
+  const int64_t size = static_cast<int64_t>(p.M) * p.N;
   if (i >= size) return;
-  const int64_t m = i / (p.N / V);
-  const int n = static_cast<int>(i - m * (p.N / V)) * V;
-  const vec* part = reinterpret_cast<const vec*>(p.partial) + i;
-  vec s = 0.0f;
+  const int64_t m = i / p.N;
+  const int n = static_cast<int>(i - m * p.N);
+  const float* part = p.partial + i;
+  float s = 0.0f;
   for (int j0 = 0; j0 < splits; j0 += kSumBatch) {
-    vec a[kSumBatch];
+    float a[kSumBatch];
 #pragma unroll
-    for (int u = 0; u < kSumBatch; ++u) a[u] = j0 + u < splits ? part[(j0 + u) * size] : vec(0.0f);
+    for (int u = 0; u < kSumBatch; ++u) a[u] = j0 + u < splits ? part[(j0 + u) * size] : 0.0f;
 #pragma unroll
-    for (int u = 0; u < kSumBatch; ++u)
-#pragma unroll
-      for (int e = 0; e < V; ++e) s[e] += a[u][e];
+    for (int u = 0; u < kSumBatch; ++u) s += a[u];
   }
-  uint16_t* o = p.out + m * p.out_stride + n;
-#pragma unroll
-  for (int e = 0; e < V; ++e) o[e] = f32_to_bf16(p.bias ? s[e] + bf16_to_f32(p.bias[n + e]) : s[e]);
+  p.out[m * p.out_stride + n] = f32_to_bf16(p.bias ? s + bf16_to_f32(p.bias[n]) : s);
 }
 
 // Rows of x a workgroup stages, ranges of K, and waves that share a tile of weight
@@ -740,8 +736,7 @@ extern "C" int nva_linear_w4(const void* x, int64_t x_row_stride, const void* qw
     default: status = launch_shared<64>(p, plan, s); break;
   }
   if (status != NVA_OK || plan.splits == 1) return status;
-  const int64_t threads = static_cast<int64_t>(rows) * n / (n % 4 == 0 ? 4 : 1);
-  auto* sum = n % 4 == 0 ? linear_w4_sum_kernel<4> : linear_w4_sum_kernel<1>;
-  sum<<<static_cast<uint32_t>((threads + 255) / 256), 256, 0, s>>>(p, plan.splits);
+  const int64_t blocks = (static_cast<int64_t>(rows) * n + 255) / 256;
+  linear_w4_sum_kernel<<<static_cast<uint32_t>(blocks), 256, 0, s>>>(p, plan.splits);
   return launch_status();
 }
