@@ -107,6 +107,20 @@ def test_linear_w4_strides_out_and_alignment(cuda):
     assert (out[:, :2] == 7).all() and (out[:, 38:] == 7).all()
 
 
+def test_linear_w4_codes_past_two_to_the_31_bytes(cuda):
+    n, k, group = 215000, 20480, 128
+    qw = torch.randint(0, 256, (n, k // 2), generator=gen(11), device="cuda", dtype=torch.uint8)
+    assert qw.numel() > 2 ** 31
+    s = (torch.randn(k // group, n, generator=gen(12), device="cuda") * 0.02).to(BF16)
+    for rows in (3, 20):
+        x = torch.randn(rows, k, generator=gen(rows), device="cuda").to(BF16)
+        got = K.linear_w4(x, qw, s)
+        for at in (0, 104800, n - 48):
+            part = slice(at, at + 48)
+            want, tol = w4_reference(x, qw[part], s[:, part], None, None)
+            close(got[:, part], want, tol)
+
+
 @pytest.mark.parametrize("rows,k", [(33, 288), (64, 256), (17, 5440)])
 def test_linear_w4_rows_far_apart(cuda, rows, k):
     """Columns of a wide tensor up to the largest stride that the kernel takes
