@@ -18,7 +18,6 @@ import os
 import random
 import sys
 import zlib
-from functools import lru_cache
 from types import SimpleNamespace
 
 import torch
@@ -33,7 +32,6 @@ THETA = 1000000.0
 TRAINED = 40960             # positions a model was trained on, before scaling
 
 
-@lru_cache(maxsize=1)
 def _kernels():
     path = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))),
                         "extend-nano-vllm_amd")
