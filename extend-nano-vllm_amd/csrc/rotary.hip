@@ -17,6 +17,8 @@
 // (4.6-5.0 TB/s; a copy reaches 5.07), 384 tokens 4.0 us, one token 2.4.  A
 // workgroup takes a token: its threads first form one angle each, shared by all
 // heads through LDS, then turn pairs 16 bytes at a time.
+#include <type_traits>
+
 #include "common.h"
 
 namespace nva {
@@ -38,6 +40,7 @@ struct RotaryParams {
   Heads q, k;
   float factor;
   int32_t num_tokens, hq, heads;       // heads: queries and keys
+  int32_t head_dim;
   int32_t pairs, per_head;             // units of a head: pair chunks, then tail chunks
   int32_t pair_chunks;
 };
@@ -79,11 +82,21 @@ template <typename T, int N>
 struct alignas(sizeof(T) * N < 16 ? sizeof(T) * N : 16) Pack {
   T v[N];
 };
+// two elements wherever they lie
+template <typename T>
+struct Two {
+  T v[2];
+};
 
 // P: pairs of a unit.  Half layout: P elements at i and P at i + pairs;
-// interleaved: 2 P elements side by side.  A tail unit copies 2 P elements.
+// interleaved: 2 P elements side by side.  A tail unit copies 2 P elements in
+// accesses of the pairs' size; units of one pair take any address, and the last
+// of an odd tail copies one element.
 template <typename T, int P, bool INTERLEAVED>
 __global__ void __launch_bounds__(kThreads) rotary_kernel(RotaryParams p) {
+  using Unit = std::conditional_t<P == 1, Two<T>, Pack<T, 2 * P>>;   // of the interleaved layout
+  using Piece = std::conditional_t<INTERLEAVED && P != 1, Unit, Pack<T, P>>;
+  constexpr int kPiece = sizeof(Piece) / sizeof(T);
   __shared__ float2 turn[kMaxPairs];
   const int64_t t = blockIdx.x;
   const double position = static_cast<double>(p.positions[t]);
@@ -101,19 +114,22 @@ __global__ void __launch_bounds__(kThreads) rotary_kernel(RotaryParams p) {
     T* out = static_cast<T*>(hd.out) + t * hd.out_row + h * hd.out_head;
     if (c >= p.pair_chunks) {
       const int d = 2 * p.pairs + 2 * P * (c - p.pair_chunks);
-      *reinterpret_cast<Pack<T, 2 * P>*>(out + d) = *reinterpret_cast<const Pack<T, 2 * P>*>(in + d);
+#pragma unroll
+      for (int e = 0; e < 2 * P; e += kPiece)
+        if (P > 1 || e == 0 || d + e < p.head_dim)
+          *reinterpret_cast<Piece*>(out + d + e) = *reinterpret_cast<const Piece*>(in + d + e);
       continue;
     }
     const float2* cs = turn + P * c;
     if constexpr (INTERLEAVED) {
-      Pack<T, 2 * P> v = *reinterpret_cast<const Pack<T, 2 * P>*>(in + 2 * P * c);
+      Unit v = *reinterpret_cast<const Unit*>(in + 2 * P * c);
 #pragma unroll
       for (int e = 0; e < P; ++e) {
         const float x = to_f32(v.v[2 * e]), y = to_f32(v.v[2 * e + 1]);
         v.v[2 * e] = from_f32<T>(x * cs[e].x - y * cs[e].y);
         v.v[2 * e + 1] = from_f32<T>(y * cs[e].x + x * cs[e].y);
       }
-      *reinterpret_cast<Pack<T, 2 * P>*>(out + 2 * P * c) = v;
+      *reinterpret_cast<Unit*>(out + 2 * P * c) = v;
     } else {
       Pack<T, P> a = *reinterpret_cast<const Pack<T, P>*>(in + P * c);
       Pack<T, P> b = *reinterpret_cast<const Pack<T, P>*>(in + p.pairs + P * c);
@@ -150,7 +166,7 @@ void launch(RotaryParams p, bool interleaved, int32_t tail, bool in_place, hipSt
   }
   p.pair_chunks = p.pairs / P;
   // in place the tail is where it belongs
-  p.per_head = p.pair_chunks + (in_place ? 0 : tail / (2 * P));
+  p.per_head = p.pair_chunks + (in_place ? 0 : (tail + 2 * P - 1) / (2 * P));
   const int32_t grid = p.num_tokens;
   if (interleaved) {
     if constexpr (2 * P * sizeof(T) <= 16) rotary_kernel<T, P, true><<<grid, kThreads, 0, s>>>(p);
@@ -189,6 +205,7 @@ extern "C" int nva_rotary_embedding(
   p.num_tokens = num_tokens;
   p.hq = num_q_heads;
   p.heads = num_q_heads + num_k_heads;
+  p.head_dim = head_dim;
   p.pairs = rotary_dim / 2;
   const int32_t tail = head_dim - rotary_dim;
   auto same = [](const Heads& h) { return h.in == h.out && h.in_row == h.out_row && h.in_head == h.out_head; };

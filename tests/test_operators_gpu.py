@@ -305,6 +305,51 @@ def test_rotary_views_and_in_place(cuda, dtype, interleaved, rot):
     assert torch.equal(qkv[:, (hq + hk) * d:], before[:, (hq + hk) * d:])
 
 
+@pytest.mark.parametrize("interleaved", [False, True])
+@pytest.mark.parametrize("dtype", [BF16, torch.float16, torch.float32])
+@pytest.mark.parametrize("t,hq,hk,d,rot", [
+    (3, 2, 1, 65, 64), (1, 1, 1, 3, 2), (5, 4, 2, 33, 32), (4, 3, 1, 129, 64), (2, 2, 2, 1023, 512),
+    (7, 5, 1, 67, 6), (260, 8, 1, 65, 62)])
+def test_rotary_odd_heads_are_whole(cuda, interleaved, dtype, t, hq, hk, d, rot):
+    g = gen(d + rot)
+    q = torch.randn(t, hq, d, generator=g, device="cuda").to(dtype)
+    k = torch.randn(t, hk, d, generator=g, device="cuda").to(dtype)
+    pos = torch.randint(0, 40960, (t,), generator=g, device="cuda")
+    freq = rope_frequencies(rot, 10000.0)[0].cuda()
+    # one element more behind each head, which stays
+    qo, ko = (torch.full((t, h, d + 1), float("nan"), dtype=dtype, device="cuda") for h in (hq, hk))
+    K.rotary_embedding(pos, q, k, freq, interleaved, q_out=qo[..., :d], k_out=ko[..., :d])
+    for x, out in ((q, qo), (k, ko)):
+        close(out[..., :d], *rotary_reference(x, pos, freq, interleaved, 1.0))
+        assert torch.equal(out[..., rot:d], x[..., rot:]) and out[..., d].isnan().all()
+    # in place, whole heads side by side
+    both = torch.cat([q, k], 1)
+    K.rotary_embedding(pos, both[:, :hq], both[:, hq:], freq, interleaved, q_out=both[:, :hq],
+                       k_out=both[:, hq:])
+    assert torch.equal(both, torch.cat([qo[..., :d], ko[..., :d]], 1))
+
+
+@pytest.mark.parametrize("interleaved", [False, True])
+@pytest.mark.parametrize("dtype", [BF16, torch.float16, torch.float32])
+def test_rotary_heads_at_every_alignment(cuda, interleaved, dtype):
+    """Heads that begin 1 to 16 elements behind a 16-byte border, with and without
+    elements behind the rotated ones."""
+    t, h = 5, 3
+    for d, rot in ((64, 32), (64, 64), (40, 16), (24, 8)):
+        pos = torch.randint(0, 40960, (t,), generator=gen(d), device="cuda")
+        freq = rope_frequencies(rot, 10000.0)[0].cuda()
+        for at in (1, 2, 4, 8, 16):
+            for gap in (0, 1, 2, 4, 8):
+                row = torch.randn(t, h, d + gap, generator=gen(at), device="cuda").to(dtype)
+                store = torch.zeros(row.numel() + at, dtype=dtype, device="cuda")
+                x = store[at:].view(t, h, d + gap)
+                x.copy_(row)
+                out = torch.full_like(store, float("nan"))[at:].view(t, h, d + gap)
+                K.rotary_embedding(pos, x[..., :d], None, freq, interleaved, q_out=out[..., :d])
+                close(out[..., :d], *rotary_reference(x[..., :d], pos, freq, interleaved, 1.0))
+                assert out[..., d:].isnan().all()
+
+
 def test_rotary_nothing_to_do(cuda):
     freq = rope_frequencies(64, 1e4)[0].cuda()
     x = torch.empty(0, 4, 64, dtype=BF16, device="cuda")
