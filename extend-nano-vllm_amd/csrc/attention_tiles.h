@@ -54,6 +54,13 @@ struct AttnParams {
 
 __device__ __forceinline__ float exp2f_fast(float x) { return __builtin_amdgcn_exp2f(x); }
 
+// Log-sum-exp (log2 domain) of a part of a row's keys, from its running maximum
+// and sum: -inf where the row sees no key of it (the sum is 0; the largest score
+// of those it sees leaves at least 1), NaN where a score was NaN or +inf.
+__device__ __forceinline__ float part_lse(float m, float sum) {
+  return sum == 0.0f ? -INFINITY : m + __log2f(sum);
+}
+
 // Reductions over the lane pairs (l, l ^ 16) and (l, l ^ 32), every lane
 // receiving the pair's result.  gfx950's v_permlane16_swap /
 // v_permlane32_swap with both operands x leave the pair's two values, the
@@ -666,7 +673,7 @@ __device__ __forceinline__ void attend_segment(const AttnParams& p, uint32_t* vs
           *reinterpret_cast<float4*>(wo) = make_float4(o[0], o[1], o[2], o[3]);
           *reinterpret_cast<float4*>(wo + 4) = make_float4(o[4], o[5], o[6], o[7]);
           // log-sum-exp (log2 domain) of the column for combine_kernel
-          if (pp == 0 && g == 0) p.ws_lse[slot] = lsum > 0.0f ? M + __log2f(lsum) : -INFINITY;
+          if (pp == 0 && g == 0) p.ws_lse[slot] = part_lse(M, lsum);
         }
       }
     }
@@ -708,7 +715,7 @@ __device__ __forceinline__ void attend_segment(const AttnParams& p, uint32_t* vs
         }
       }
       // log-sum-exp (log2 domain) of the column for combine_kernel
-      if (nsplit > 1 && g == 0) p.ws_lse[slot] = lsum > 0.0f ? m_run[nt] + __log2f(lsum) : -INFINITY;
+      if (nsplit > 1 && g == 0) p.ws_lse[slot] = part_lse(m_run[nt], lsum);
     }
   }
 }
@@ -971,9 +978,50 @@ __device__ __forceinline__ void attend_tile(const AttnParams& p, uint32_t* slots
           *reinterpret_cast<float4*>(wo + 4) = make_float4(o[4], o[5], o[6], o[7]);
         }
       }
-      if (nsplit > 1 && g == 0) p.ws_lse[slot] = lsum > 0.0f ? m_run[nt] + __log2f(lsum) : -INFINITY;
+      if (nsplit > 1 && g == 0) p.ws_lse[slot] = part_lse(m_run[nt], lsum);
     }
   }
+}
+
+// ---------------------------------------------------------------- joining parts
+
+// Elements 4 d4 .. 4 d4 + 3 of a row and head's output from its `parts` parts (the
+// first at slot `base`): sum w o / sum w with w = exp2(lse - max lse), kJoinBatch
+// loads at a time folded into a running maximum, weight and sum.  Parts without a
+// visible key have no weight; without any the row is zero.  A NaN part makes the
+// row NaN, whatever the others hold: the maximum passes over it, its weight is NaN.
+constexpr int kJoinBatch = 8;
+__device__ __forceinline__ float4 join_parts(const AttnParams& p, int64_t base, int parts, int d4) {
+  float M = -INFINITY, wsum = 0.0f;
+  float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+  for (int s0 = 0; s0 < parts; s0 += kJoinBatch) {
+    float lse[kJoinBatch];
+    float4 v[kJoinBatch];
+#pragma unroll
+    for (int u = 0; u < kJoinBatch; ++u) {
+      const bool in = s0 + u < parts;
+      lse[u] = in ? p.ws_lse[base + s0 + u] : -INFINITY;
+      v[u] = in ? *reinterpret_cast<const float4*>(p.ws_o + (base + s0 + u) * kD + 4 * d4)
+                : make_float4(0.f, 0.f, 0.f, 0.f);
+    }
+    float mb = M;
+#pragma unroll
+    for (int u = 0; u < kJoinBatch; ++u) mb = fmaxf(mb, lse[u]);
+    const float msub = mb == -INFINITY ? 0.0f : mb;
+    const float r = M == -INFINITY ? 0.0f : exp2f_fast(M - msub);
+    wsum *= r;
+    o.x *= r; o.y *= r; o.z *= r; o.w *= r;
+#pragma unroll
+    for (int u = 0; u < kJoinBatch; ++u) {
+      if (lse[u] == -INFINITY) v[u] = make_float4(0.f, 0.f, 0.f, 0.f);   // whatever is there
+      const float w = lse[u] == -INFINITY ? 0.0f : exp2f_fast(lse[u] - msub);
+      wsum += w;
+      o.x += w * v[u].x; o.y += w * v[u].y; o.z += w * v[u].z; o.w += w * v[u].w;
+    }
+    M = mb;
+  }
+  const float inv = wsum == 0.0f ? 0.0f : 1.0f / wsum;
+  return make_float4(o.x * inv, o.y * inv, o.z * inv, o.w * inv);
 }
 
 // ---------------------------------------------------------------- 32-row waves

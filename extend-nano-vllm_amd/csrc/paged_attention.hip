@@ -587,7 +587,7 @@ paged_attention_wide_kernel(AttnParams p) {
           *reinterpret_cast<float4*>(wo + 32 * dt + 8 * b + 4 * h) =
               make_float4(acc[dt][4 * b] * inv, acc[dt][4 * b + 1] * inv, acc[dt][4 * b + 2] * inv,
                           acc[dt][4 * b + 3] * inv);
-      if (h == 0) p.ws_lse[slot] = lsum > 0.0f ? m_run + __log2f(lsum) : -INFINITY;
+      if (h == 0) p.ws_lse[slot] = part_lse(m_run, lsum);
     }
   }
   // by the threads that get here: the other key group has returned
@@ -691,9 +691,8 @@ paged_attention_stream_kernel(AttnParams p) {
 // 256 (head, 4-element) slices y*256 .. of the row; each thread owns one
 // slice.  The attention kernel recorded each row's split count, so a row
 // costs one dependent load before its partials; every thread issues the
-// loads of up to kCombineBatch splits at once (partials are laid out
-// [row][head][split][d]) and merges batches with a running log-sum-exp.
-constexpr int kCombineBatch = 8;
+// loads of up to kJoinBatch splits at once (partials are laid out
+// [row][head][split][d]).
 __global__ void __launch_bounds__(kCombineThreads)
 combine_kernel(AttnParams p) {
   const int t = blockIdx.x;
@@ -709,37 +708,10 @@ combine_kernel(AttnParams p) {
   if (idx >= p.hq * (kD / 4)) return;
   const int h = idx / (kD / 4), d4 = idx % (kD / 4);
   const int64_t base = (static_cast<int64_t>(t) * p.hq + h) * p.max_splits;
-  float M = -INFINITY, wsum = 0.0f;
-  float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
-  for (int s0 = 0; s0 < nsplit; s0 += kCombineBatch) {
-    float lse[kCombineBatch];
-    float4 v[kCombineBatch];
-#pragma unroll
-    for (int u = 0; u < kCombineBatch; ++u) {
-      const bool in = s0 + u < nsplit;
-      lse[u] = in ? p.ws_lse[base + s0 + u] : -INFINITY;
-      v[u] = in ? *reinterpret_cast<const float4*>(p.ws_o + (base + s0 + u) * kD + 4 * d4)
-                : make_float4(0.f, 0.f, 0.f, 0.f);
-    }
-    float mb = M;
-#pragma unroll
-    for (int u = 0; u < kCombineBatch; ++u) mb = fmaxf(mb, lse[u]);
-    if (mb == -INFINITY) continue;
-    const float r = M == -INFINITY ? 0.0f : exp2f_fast(M - mb);
-    wsum *= r;
-    o.x *= r; o.y *= r; o.z *= r; o.w *= r;
-#pragma unroll
-    for (int u = 0; u < kCombineBatch; ++u) {
-      const float w = lse[u] == -INFINITY ? 0.0f : exp2f_fast(lse[u] - mb);
-      wsum += w;
-      o.x += w * v[u].x; o.y += w * v[u].y; o.z += w * v[u].z; o.w += w * v[u].w;
-    }
-    M = mb;
-  }
-  const float inv = wsum > 0.0f ? 1.0f / wsum : 0.0f;
+  const float4 o = join_parts(p, base, nsplit, d4);
   uint16_t* op = p.out + static_cast<int64_t>(t) * p.out_row_stride +
                  static_cast<int64_t>(h) * p.out_head_stride + 4 * d4;
-  *reinterpret_cast<uint2*>(op) = make_uint2(pack_bf16(o.x * inv, o.y * inv), pack_bf16(o.z * inv, o.w * inv));
+  *reinterpret_cast<uint2*>(op) = make_uint2(pack_bf16(o.x, o.y), pack_bf16(o.z, o.w));
 }
 
 // query positions per workgroup: as many as fit 64 tile rows (>= 1)

@@ -343,7 +343,7 @@ __device__ __forceinline__ void wide_unit(const AttnParams& p, uint32_t* lds, co
     const float4 o = *reinterpret_cast<const float4*>(park + (2 * i + h) * kParkPitch + 4 * col);
     if (r < rows) *reinterpret_cast<float4*>(p.ws_o + slot_of(r) * kD + 4 * col) = o;
   }
-  if (n < rows && h == 0) p.ws_lse[slot_of(n)] = lsum > 0.0f ? m_run + __log2f(lsum) : -INFINITY;
+  if (n < rows && h == 0) p.ws_lse[slot_of(n)] = part_lse(m_run, lsum);
 }
 
 // OWN: how the own keys' units run: tiles of 16 (1) or 32 (2) rows on
@@ -417,10 +417,8 @@ __global__ void __launch_bounds__(kThreads, 2) shared_prefix_kernel(PrefixParams
   }
 }
 
-// The join.  A thread owns four head_dim elements of one (token, head) and folds
-// its parts, kBatch loads at a time, into a running maximum, weight and sum.
+// The join.  A thread owns four head_dim elements of one (token, head).
 constexpr int kJoinThreads = 256;
-constexpr int kBatch = 8;
 __global__ void __launch_bounds__(kJoinThreads) join_kernel(PrefixParams pp) {
   const AttnParams& p = pp.a;
   const int t = blockIdx.x;
@@ -435,37 +433,10 @@ __global__ void __launch_bounds__(kJoinThreads) join_kernel(PrefixParams pp) {
   own = own < pp.own_parts ? own : pp.own_parts;
   const int parts = own < 0 ? 0 : pp.prefix_parts + own;
   const int64_t base = (static_cast<int64_t>(t) * p.hq + h) * p.max_splits;
-  float M = -INFINITY, wsum = 0.0f;
-  float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
-  for (int s0 = 0; s0 < parts; s0 += kBatch) {
-    float lse[kBatch];
-    float4 v[kBatch];
-#pragma unroll
-    for (int u = 0; u < kBatch; ++u) {
-      const bool in = s0 + u < parts;
-      lse[u] = in ? p.ws_lse[base + s0 + u] : -INFINITY;
-      v[u] = in ? *reinterpret_cast<const float4*>(p.ws_o + (base + s0 + u) * kD + 4 * d4)
-                : make_float4(0.f, 0.f, 0.f, 0.f);
-    }
-    float mb = M;
-#pragma unroll
-    for (int u = 0; u < kBatch; ++u) mb = fmaxf(mb, lse[u]);
-    if (mb == -INFINITY) continue;
-    const float r = M == -INFINITY ? 0.0f : exp2f_fast(M - mb);
-    wsum *= r;
-    o.x *= r; o.y *= r; o.z *= r; o.w *= r;
-#pragma unroll
-    for (int u = 0; u < kBatch; ++u) {
-      const float w = lse[u] == -INFINITY ? 0.0f : exp2f_fast(lse[u] - mb);
-      wsum += w;
-      o.x += w * v[u].x; o.y += w * v[u].y; o.z += w * v[u].z; o.w += w * v[u].w;
-    }
-    M = mb;
-  }
-  const float inv = wsum > 0.0f ? 1.0f / wsum : 0.0f;
+  const float4 o = join_parts(p, base, parts, d4);
   uint16_t* op = p.out + static_cast<int64_t>(t) * p.out_row_stride +
                  static_cast<int64_t>(h) * p.out_head_stride + 4 * d4;
-  *reinterpret_cast<uint2*>(op) = make_uint2(pack_bf16(o.x * inv, o.y * inv), pack_bf16(o.z * inv, o.w * inv));
+  *reinterpret_cast<uint2*>(op) = make_uint2(pack_bf16(o.x, o.y), pack_bf16(o.z, o.w));
 }
 
 // Compute units of the current device (cached per device; 256 when the query fails).

@@ -225,6 +225,8 @@ int nva_argmax_rows(const void *logits, int64_t row_stride, int32_t vocab, int32
  *   softmax_scale multiplies q.k; for FP8 caches the scores are also
  *      multiplied by *k_scale and the output by *v_scale (NULL = 1.0), as in
  *      the reference's FP8 decode kernel; bf16 caches ignore the scales.
+ *   A NaN score (of a NaN in a query row, or in a key that the row sees) makes
+ *      the row NaN, however its keys are split.
  *   GQA: query head h reads kv head h / (num_q_heads / num_kv_heads).
  *   head_dim must be 128, block_size a multiple of 32 and
  *      num_q_heads / num_kv_heads <= 64; any query length is accepted.

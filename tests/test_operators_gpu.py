@@ -548,6 +548,60 @@ def test_shared_prefix_blocks_outside_the_cache_hold_no_keys(cuda):
     assert (got == 0).all()
 
 
+def put(pages, at, value):
+    """pages[at] = value, FP8 pages too (which hold no infinity: NaN)."""
+    if pages.dtype == FP8:
+        pages.view(torch.uint8)[at] = 0x7F
+    else:
+        pages[at] = value
+
+
+NAN_CASES = [   # the last keys' units on 16, 32, 64 and 128 rows; one part, some, more than a join's batch
+    ([1] * 4, [70, 100, 90, 300], 64, 8, 4), ([1] * 3, [8000, 9000, 8200], 7936, 4, 1),
+    ([4, 2, 3], [900, 540, 2700], 512, 8, 1), ([8, 8], [600, 2000], 512, 64, 8),
+    ([40, 3], [600, 3000], 512, 16, 4), ([1] * 70, [530 + i for i in range(70)], 512, 8, 2)]
+
+
+@pytest.mark.parametrize("fp8", [False, True])
+@pytest.mark.parametrize("rows,keys,prefix,hq,hkv", NAN_CASES)
+@pytest.mark.parametrize("shared", [True, False])
+def test_attention_nan_reaches_the_rows_that_see_it(cuda, shared, rows, keys, prefix, hq, hkv, fp8):
+    q, kc, vc, cu_q, cu_k, table = pages_case(rows, keys, prefix, hq, hkv, fp8=fp8, seed=prefix)
+    want, tol = prefix_reference(q, kc, vc, rows, keys, table, SCALE)
+    group, t = hq // hkv, sum(rows)
+    one = torch.ones(1, device="cuda")
+
+    def check(q, kc, vc, bad):
+        if shared:
+            got = K.shared_prefix_attention_varlen(q, kc, vc, cu_q, cu_k, max(rows), max(keys), prefix,
+                                                   SCALE, table, k_scale=one, v_scale=one)
+        else:
+            got = K.paged_attention_varlen(q, kc, vc, cu_q, cu_k, max(rows), max(keys), SCALE, table,
+                                           k_scale=one, v_scale=one)
+        got = got.cpu()
+        assert got[bad].isnan().all()
+        if not bad.all():
+            close(got[~bad], want[~bad], tol[~bad])
+
+    bad = torch.zeros(t, hq, dtype=torch.bool)
+    bad[::3, 1] = True
+    broken = q.clone()
+    broken[::3, 1, 5] = float("nan")
+    check(broken, kc, vc, bad)
+    # a key that all see, one of the prefix's last, and one of the last sequence's own
+    for seq, key in ((0, 3), (0, prefix - 1), (len(keys) - 1, keys[-1] - rows[-1])):
+        broken, values = kc.clone(), vc.clone()      # of the same strides
+        block = (table[seq:seq + 1] if seq else table)[:, key // 256].long()
+        put(broken, (block, key % 256, 0, 9), float("nan"))
+        bad = torch.zeros(t, hq, dtype=torch.bool)
+        start = 0
+        for i, (r, n) in enumerate(zip(rows, keys)):
+            if i == seq or seq == 0:
+                bad[start + max(0, key - (n - r)):start + r, :group] = True
+            start += r
+        check(q, broken, values, bad)
+
+
 def test_shared_prefix_clips_like_paged_attention(cuda):
     # longer than the bounds on the device: rows past max_seqlen_q are zeros,
     # keys past max_seqlen_k unseen
