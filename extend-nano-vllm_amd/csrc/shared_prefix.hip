@@ -43,6 +43,11 @@ struct PrefixParams {
   int32_t prefix_units, own_units;                   // per kv head
 };
 
+// Ones over the bf16 values of a dword that are finite.
+__device__ __forceinline__ uint32_t finite_mask(uint32_t w) {
+  return ((w & 0x7F80u) == 0x7F80u ? 0u : 0xFFFFu) | ((w & 0x7F800000u) == 0x7F800000u ? 0u : 0xFFFF0000u);
+}
+
 // A tile of query rows of one kv head (positions tok0 .. tok0 + jn - 1 of the
 // batch, all heads of the group) against the keys [kv_begin, kv_end) of a block
 // table, 64 keys a step; the part goes to the workspace.
@@ -59,9 +64,15 @@ struct PrefixParams {
 //   * K/V go through registers two steps ahead and one of two LDS buffers one
 //     step ahead, one barrier a step.  FP8 pages become bf16 on the way.
 //   * The part leaves through LDS as whole rows of 512 bytes.
-// last_key[j]: the last key that position tok0 + j sees (less than 0: none).
+//   * A hidden key's weight of zero does not keep an infinity or NaN in its V out of
+//     a product (0 * inf is NaN).  Tiles with keys that some row does not see are
+//     staged with zeros in place of such elements; where there was one (a flag, which
+//     the caller has cleared), they are added at the end, read again, to the rows
+//     that see them.  Rows that see no key of the range have no part in the join.
+// last_key[j]: the last key that position tok0 + j sees (less than 0: none);
+// last_key[kTileRows]: the flag.
 template <bool HALVES, bool FP8>
-__device__ __forceinline__ void wide_unit(const AttnParams& p, uint32_t* lds, const int32_t* last_key,
+__device__ __forceinline__ void wide_unit(const AttnParams& p, uint32_t* lds, int32_t* last_key,
                                           const int kvh, const int tok0, const int jn,
                                           const int kv_begin, const int kv_end, const int part,
                                           const int32_t* table) {
@@ -106,6 +117,12 @@ __device__ __forceinline__ void wide_unit(const AttnParams& p, uint32_t* lds, co
     most = b > most ? b : most;
   }
   const int wave_full = __builtin_amdgcn_readfirstlane(least) + 1;   // keys below it are seen by every row
+  // of this lane's positions that see a key of the range, the one that sees the fewest
+  int seen = 0x7FFFFFFF;
+  for (int j = lane; j < jn; j += kWave) {
+    const int k = last_key[j];
+    if (k >= kv_begin && k < seen) seen = k;
+  }
   // keys from it on by none
   const int wave_end = 32 * rw < rows ? __builtin_amdgcn_readfirstlane(most) + 1 : 0;
 
@@ -175,20 +192,32 @@ __device__ __forceinline__ void wide_unit(const AttnParams& p, uint32_t* lds, co
           uint4, __builtin_amdgcn_raw_buffer_load_b128(upper[i] ? v1 : v0, goff[i], 0, 0));
     }
   };
-  auto stage = [&](const Tile& t, int b) {
+  auto stage = [&](const Tile& t, int b, int key0) {
     uint32_t* base = lds + b * kWideBuf;
+    const int top = key0 + kWideKeys < kv_end ? key0 + kWideKeys - 1 : kv_end - 1;
+    const bool hidden = __any(seen < top);
+    bool bad = false;
+    auto put_v = [&](uint32_t* at, uint4 v) {
+      if (hidden) {
+        const uint4 m = make_uint4(finite_mask(v.x), finite_mask(v.y), finite_mask(v.z), finite_mask(v.w));
+        bad |= (m.x & m.y & m.z & m.w) != 0xFFFFFFFFu;
+        v = make_uint4(v.x & m.x, v.y & m.y, v.z & m.z, v.w & m.w);
+      }
+      *reinterpret_cast<uint4*>(at) = v;
+    };
 #pragma unroll
     for (int i = 0; i < kPer; ++i) {
       if constexpr (FP8) {
         *reinterpret_cast<bf16x8_t*>(base + kdst[i]) = fp8x8_to_bf16(make_uint2(t.k[i].x, t.k[i].y));
         *reinterpret_cast<bf16x8_t*>(base + kdst[i] + 4) = fp8x8_to_bf16(make_uint2(t.k[i].z, t.k[i].w));
-        *reinterpret_cast<bf16x8_t*>(base + vdst[i]) = fp8x8_to_bf16(make_uint2(t.v[i].x, t.v[i].y));
-        *reinterpret_cast<bf16x8_t*>(base + vdst[i] + 4) = fp8x8_to_bf16(make_uint2(t.v[i].z, t.v[i].w));
+        put_v(base + vdst[i], __builtin_bit_cast(uint4, fp8x8_to_bf16(make_uint2(t.v[i].x, t.v[i].y))));
+        put_v(base + vdst[i] + 4, __builtin_bit_cast(uint4, fp8x8_to_bf16(make_uint2(t.v[i].z, t.v[i].w))));
       } else {
         *reinterpret_cast<uint4*>(base + kdst[i]) = t.k[i];
-        *reinterpret_cast<uint4*>(base + vdst[i]) = t.v[i];
+        put_v(base + vdst[i], t.v[i]);
       }
     }
+    if (bad) last_key[kTileRows] = 1;
   };
 
   float m_run = -INFINITY, l_run = 0.0f;
@@ -274,14 +303,14 @@ __device__ __forceinline__ void wide_unit(const AttnParams& p, uint32_t* lds, co
   const int ntiles = (kv_end - kv_begin + kWideKeys - 1) / kWideKeys;
   Tile t;
   load_tile(t);
-  stage(t, 0);
+  stage(t, 0, kv_begin);
   int valid = t.valid;
   load_tile(t);
   __syncthreads();
   for (int c = 0; c < ntiles; ++c) {
     compute(kv_begin + c * kWideKeys, valid, c & 1);
     if (c + 1 < ntiles) {
-      stage(t, (c + 1) & 1);
+      stage(t, (c + 1) & 1, kv_begin + (c + 1) * kWideKeys);
       valid = t.valid;
       load_tile(t);
     }
@@ -323,6 +352,36 @@ __device__ __forceinline__ void wide_unit(const AttnParams& p, uint32_t* lds, co
         for (int i = 0; i < 4; ++i) acc[dt][4 * b + i] = f0 * acc[dt][4 * b + i] + f1 * o[i];
       }
   }
+  if (last_key[kTileRows]) {
+#pragma unroll 1
+    for (int key = kv_begin; key < kv_end; ++key) {
+      const int c = key / p.block_size;
+      const int raw = c < p.bt_cols ? table[c] : -1;
+      if (raw < 0 || raw >= p.num_blocks || key > lim) continue;
+      const uint8_t* row = p.v_cache + (static_cast<int64_t>(raw) * p.blk_stride +
+                                        static_cast<int64_t>(kvh) * p.head_stride +
+                                        static_cast<int64_t>(key % p.block_size) * p.tok_stride) * kEsz;
+#pragma unroll
+      for (int dt = 0; dt < 4; ++dt)
+#pragma unroll
+        for (int b = 0; b < 4; ++b) {
+          const uint8_t* at = row + (32 * dt + 8 * b + 4 * h) * kEsz;
+          if constexpr (FP8) {
+            const uint32_t w = *reinterpret_cast<const uint32_t*>(at);
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+              if ((w >> (8 * i) & 0x7Fu) == 0x7Fu) acc[dt][4 * b + i] = __builtin_nanf("");
+          } else {
+            const uint2 v = *reinterpret_cast<const uint2*>(at);
+            const uint32_t x = v.x & ~finite_mask(v.x), y = v.y & ~finite_mask(v.y);
+            acc[dt][4 * b] += __uint_as_float(x << 16);
+            acc[dt][4 * b + 1] += __uint_as_float(x & 0xFFFF0000u);
+            acc[dt][4 * b + 2] += __uint_as_float(y << 16);
+            acc[dt][4 * b + 3] += __uint_as_float(y & 0xFFFF0000u);
+          }
+        }
+    }
+  }
   const float lsum = sum_xor32(l_run);
   const float inv = lsum > 0.0f ? vscale / lsum : 0.0f;
   // through the wave's own rows of LDS, then out row by row
@@ -355,7 +414,7 @@ __global__ void __launch_bounds__(kThreads, 2) shared_prefix_kernel(PrefixParams
                           : kSegDwords + OWN * 4 * kWave * 4 > kWideDwords ? kSegDwords + OWN * 4 * kWave * 4
                                                                            : kWideDwords;
   __shared__ __attribute__((aligned(16))) uint32_t lds[kDwords];
-  __shared__ int32_t last_key[kTileRows];                // of each query position of a wide tile
+  __shared__ int32_t last_key[kTileRows + 1];            // of each query position of a wide tile, and its flag
   const AttnParams& p = pp.a;
   const int kvh = blockIdx.x % p.hkv;
   const int u = blockIdx.x / p.hkv;
@@ -367,6 +426,7 @@ __global__ void __launch_bounds__(kThreads, 2) shared_prefix_kernel(PrefixParams
     const int kv_end = kv_begin + pp.prefix_split < pp.prefix ? kv_begin + pp.prefix_split : pp.prefix;
     // every position's last visible key, from the sequence that holds it
     for (int i = threadIdx.x; i < jn; i += kThreads) last_key[i] = -1;
+    if (threadIdx.x == 0) last_key[kTileRows] = 0;
     __syncthreads();
     for (int seq = p.cu_q ? static_cast<int>(threadIdx.x) : tok0 + static_cast<int>(threadIdx.x);
          seq < (p.cu_q ? p.num_seqs : tok0 + jn); seq += kThreads) {
@@ -411,6 +471,7 @@ __global__ void __launch_bounds__(kThreads, 2) shared_prefix_kernel(PrefixParams
                            pp.prefix_parts + split, 2, lane_blk);
   } else {
     for (int j = threadIdx.x; j < jn; j += kThreads) last_key[j] = L - q_len + j0 + j;
+    if (threadIdx.x == 0) last_key[kTileRows] = 0;
     __syncthreads();
     wide_unit<OWN == 3, FP8>(p, lds, last_key, kvh, q_start + j0, jn, kv_begin, kv_end,
                              pp.prefix_parts + split, p.block_tables + static_cast<int64_t>(seq) * p.bt_stride);

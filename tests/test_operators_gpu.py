@@ -616,6 +616,35 @@ def test_shared_prefix_clips_like_paged_attention(cuda):
         assert torch.equal((got == 0).all(-1), (want == 0).all(-1))
 
 
+HIDDEN_CASES = [
+    ([1] * 6, [700, 100, 6, 1, 32, 512], 512, 8, 4), ([5, 9, 3, 4], [300, 4, 3, 0], 256, 8, 4),
+    ([40, 2, 60], [520, 513, 530], 512, 8, 2), ([1] * 3, [5000, 1500, 4097], 4096, 4, 1),
+    ([1] * 90, [520 + 7 * i if i % 3 else 8 * i + 1 for i in range(90)], 512, 8, 2),
+    ([130, 3], [400, 90], 256, 16, 4)]
+
+
+@pytest.mark.parametrize("fp8", [False, True])
+@pytest.mark.parametrize("rows,keys,prefix,hq,hkv", HIDDEN_CASES)
+def test_shared_prefix_values_that_are_not_finite_stay_with_the_rows_that_see_them(
+        cuda, rows, keys, prefix, hq, hkv, fp8):
+    """An infinity or NaN in V of a shared key: rows that end before it are as if it
+    were not there, the others are not finite in that element."""
+    q, kc, vc, cu_q, cu_k, table = pages_case(rows, keys, prefix, hq, hkv, fp8=fp8, seed=prefix + 1)
+    want, tol = prefix_reference(q, kc, vc, rows, keys, table, SCALE)
+    one, group = torch.ones(1, device="cuda"), hq // hkv
+    last = torch.cat([torch.arange(n - r, n) for r, n in zip(rows, keys)])
+    bad = torch.zeros(want.shape, dtype=torch.bool)
+    for i, value in enumerate((float("nan"), float("inf"), float("-inf"))):
+        for j, key in enumerate((5, 40, prefix // 2 + 3, prefix - 1)):
+            d, head = 37 * i + 11 * j, (i + j) % hkv
+            put(vc, (table[:, key // 256].long(), key % 256, head, d), value)
+            bad[last >= key, head * group:(head + 1) * group, d] = True
+    got = K.shared_prefix_attention_varlen(q, kc, vc, cu_q, cu_k, max(rows), max(max(keys), prefix),
+                                           prefix, SCALE, table, k_scale=one, v_scale=one).cpu()
+    assert not got[bad].isfinite().any()
+    close(got[~bad], want[~bad], tol[~bad])
+
+
 def test_shared_prefix_large_scores_and_stale_slots(cuda):
     # rows whose parts differ by hundreds in the exponent, infinities and NaN in
     # slots that no row sees
