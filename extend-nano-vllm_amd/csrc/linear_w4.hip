@@ -3,12 +3,14 @@
 // with x in bf16, codes 0..15 two to a byte, group scales in bf16.
 //
 // A group's sum is formed from exact operands and scaled afterwards, so no
-// weight is ever rounded: a code c becomes the bf16 value 16 + c by placing its
-// four bits in the mantissa of 16 (one shift, one and-or for two codes), the
-// MFMA sums (16 + c) x in fp32, and with the group's sum of x
-//   sum (c - z) x = sum (16 + c) x - (16 + z) sum x.
-// Scales, the sums of x and the sum over groups are fp32, the output is rounded
-// once.
+// weight is ever rounded: a code c becomes the bf16 value 2^-12 (16 + c) by placing
+// its four bits in the mantissa of 2^-8 (one shift, one and-or for two codes), the
+// MFMA sums the products with x in fp32, and with the group's sum of 2^-8 x
+//   2^-12 sum (c - z) x = sum 2^-12 (16 + c) x - (1 + z / 16) sum 2^-8 x.
+// Scales, the sums of x and the sum over groups are fp32, brought back by 2^12 at the
+// end, and the output is rounded once.  The power of two is what keeps the up to 128
+// products of a sum finite for every finite x (128 * 31 < 2^12); sums below 2^-126
+// lose bits, which takes |x| below 2^-114.
 //
 // What bounds it: for wide outputs the codes' stream from HBM, a quarter of the
 // bf16 weights' (1 x 151936 x 4096: 58-64 us, 5.0-5.4 TB/s; a 1 GiB copy reaches
@@ -64,20 +66,22 @@ struct W4Params {
   uint32_t groups, per_group, group_magic;
 };
 
-// Two codes of a dword, nibbles S / 4 and S / 4 + 4, as the bf16 values 16 + c:
-// 16 is 0x4180 and a code's lowest bit is bit 3 of the mantissa.
+constexpr float kCodeUnit = 4096.0f;   // what a code's steps are divided by
+
+// Two codes of a dword, nibbles S / 4 and S / 4 + 4, as the bf16 values 2^-12 (16 + c):
+// 2^-8 is 0x3B80 and a code's lowest bit is bit 3 of the mantissa.
 // The two constants come in registers (one and-or; as literals they take two
 // instructions).
 struct CodeBits {
-  uint32_t mask, sixteen;
-  __device__ __forceinline__ CodeBits() : mask(0x00780078u), sixteen(0x41804180u) {
+  uint32_t mask, base;
+  __device__ __forceinline__ CodeBits() : mask(0x00780078u), base(0x3B803B80u) {
     asm volatile("" : "+s"(mask));
-    asm volatile("" : "+v"(sixteen));
+    asm volatile("" : "+v"(base));
   }
   template <int S>
   __device__ __forceinline__ uint32_t pair(uint32_t w) const {
     const uint32_t at = S < 4 ? w << 3 : w >> (S - 3);
-    return (at & mask) | sixteen;
+    return (at & mask) | base;
   }
   // Eight codes as an MFMA operand, in the order 0, 4, 1, 5, 2, 6, 3, 7.
   __device__ __forceinline__ bf16x8_t operand(uint32_t w) const {
@@ -222,9 +226,10 @@ __device__ __forceinline__ void store_tiles(const W4Params& p, const f32x4_t (&a
       const int r = 16 * m + 4 * (lane >> 4) + e;
       if (r >= M) continue;
       if (p.partial)
-        p.partial[(static_cast<int64_t>(split) * p.M + m0 + r) * p.N + n] = sum[e];
+        p.partial[(static_cast<int64_t>(split) * p.M + m0 + r) * p.N + n] = sum[e] * kCodeUnit;
       else
-        p.out[static_cast<int64_t>(m0 + r) * p.out_stride + n] = f32_to_bf16(sum[e] + bias);
+        p.out[static_cast<int64_t>(m0 + r) * p.out_stride + n] =
+            f32_to_bf16(__builtin_fmaf(sum[e], kCodeUnit, bias));
     }
   }
 }
@@ -287,7 +292,8 @@ __global__ void __launch_bounds__(kThreads, 4) linear_w4_kernel(W4Params p) {
   __syncthreads();
 
   const int xrow = RT < 16 ? m16 & (RT - 1) : m16;     // an operand row that is not staged repeats one that is
-  const bf16x8_t ones = __builtin_bit_cast(bf16x8_t, make_uint4(0x3F803F80u, 0x3F803F80u, 0x3F803F80u, 0x3F803F80u));
+  const bf16x8_t ones =                                // of 2^-8, as the codes'
+      __builtin_bit_cast(bf16x8_t, make_uint4(0x3B803B80u, 0x3B803B80u, 0x3B803B80u, 0x3B803B80u));
   const CodeBits bits;
   const f32x4_t none = f32x4_t{0.f, 0.f, 0.f, 0.f};
   f32x4_t acc[1][1] = {{none}};
@@ -329,7 +335,7 @@ __global__ void __launch_bounds__(kThreads, 4) linear_w4_kernel(W4Params p) {
 #pragma unroll
         for (int t = 0; t < 2; ++t) {
           const int i = t * (4 / PER) + d / PER;
-          const float s = __uint_as_float(sz[i] << 16), z = 16.0f + static_cast<float>(sz[i] >> 16);
+          const float s = __uint_as_float(sz[i] << 16), z = __builtin_fmaf(static_cast<float>(sz[i] >> 16), 0.0625f, 1.0f);
 #pragma unroll
           for (int e = 0; e < 4; ++e)
             acc[0][0][e] = __builtin_fmaf(s, __builtin_fmaf(-z, xsum[t][e], sum[t][e]), acc[0][0][e]);
@@ -362,8 +368,8 @@ __device__ __forceinline__ void in_order() {
 // More rows, in slabs of 64 (MT tiles of 16 staged).  A wave holds two tiles of 16
 // weight rows; the 8 / WK waves of the same step share its x, a chunk at a time in
 // LDS (with one wave a step its own), the next one or two chunks in registers.
-// The zeros' part of a sum, -scale (16 + zero) sum x, is a product of its own over
-// four groups (fp32 operands; a scale times an integer up to 31 is exact).
+// The zeros' part of a sum, -scale (1 + zero / 16) sum 2^-8 x, is a product of its own
+// over four groups (fp32 operands; a scale times up to 31 sixteenths is exact).
 template <int MT, int PER, int WK>
 __global__ void __launch_bounds__(kThreads, 2) linear_w4_slab_kernel(W4Params p) {
   constexpr int NT = 2, D = 2;
@@ -418,12 +424,12 @@ __global__ void __launch_bounds__(kThreads, 2) linear_w4_slab_kernel(W4Params p)
     if (mine + d * WK < end) codes.load(mine + d * WK, buf[d]);
   __builtin_amdgcn_sched_barrier(0);
 
-  // operand rows 4 d .. 4 d + 3 of ones: the product with x leaves the sum of x's
+  // operand rows 4 d .. 4 d + 3 of ones (2^-8, as the codes'): the product with x leaves the sum of x's
   // row l % 16 in lane quarter d, as the fp32 product takes it
   bf16x8_t ones[4];
 #pragma unroll
   for (int d = 0; d < 4; ++d) {
-    const uint32_t v = m16 / 4 == d ? 0x3F803F80u : 0u;
+    const uint32_t v = m16 / 4 == d ? 0x3B803B80u : 0u;
     ones[d] = __builtin_bit_cast(bf16x8_t, make_uint4(v, v, v, v));
   }
   const CodeBits bits;
@@ -435,13 +441,13 @@ __global__ void __launch_bounds__(kThreads, 2) linear_w4_slab_kernel(W4Params p)
     for (int m = 0; m < MT; ++m) acc[q][m] = none;
   auto compute = [&](int c, const typename Stream::Step& b) {
     uint32_t scale[NT][4];                             // of group d and, in the high half, 4 + d
-    float below[NT][kLoads];                           // -scale (16 + zero) of the lane quarter's groups
+    float below[NT][kLoads];                           // -scale (1 + zero / 16) of the lane quarter's groups
 #pragma unroll
     for (int q = 0; q < NT; ++q) {
       scale[q][0] = kLoads == 2 ? b.s[q][0] | b.s[q][kLoads - 1] << 16 : b.s[q][0];
 #pragma unroll
       for (int i = 0; i < kLoads; ++i)
-        below[q][i] = -__uint_as_float(b.s[q][i] << 16) * (16.0f + static_cast<float>(b.z[q][i]));
+        below[q][i] = -__uint_as_float(b.s[q][i] << 16) * __builtin_fmaf(static_cast<float>(b.z[q][i]), 0.0625f, 1.0f);
       if constexpr (kGroups >= 4) {
         broadcast(scale[q]);
       } else {

@@ -480,8 +480,9 @@ int nva_linear(const void *x, int64_t x_row_stride, const void *w, void *out,
  * out[m, j] = bf16(sum_i x[m, i] * (code[j, i] - zero[i / group, j]) *
  *                  scale[i / group, j] + bias[j])
  *   in fp32: a group's sum is formed from the exact codes and then scaled, so
- *   a weight is never rounded.  A row of x that holds an infinity or a NaN
- *   comes out NaN; other rows are not touched by it.
+ *   a weight is never rounded.  Any finite x: no sum within a group overflows.
+ *   A row of x that holds an infinity or a NaN comes out NaN; other rows are not
+ *   touched by it.
  * x: bf16 [rows, k], row stride x_row_stride; qweight: uint8 [n, k / 2]
  *   contiguous, element 2 i in the low and 2 i + 1 in the high half of byte i;
  *   scales: bf16 [k / group, n] contiguous; zeros: uint8 [k / group, n]

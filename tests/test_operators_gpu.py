@@ -157,6 +157,22 @@ def test_linear_w4_a_bad_row_stays_alone(cuda):
     close(got[keep], want[keep], tol[keep])
 
 
+@pytest.mark.parametrize("rows,n,k,group", [
+    (1, 40, 256, 128), (4, 130, 1024, 32), (9, 64, 4096, 64), (16, 70, 8192, 128), (17, 100, 1024, 128),
+    (33, 72, 2048, 32), (64, 130, 4096, 64), (70, 40, 672, 96)])
+@pytest.mark.parametrize("zeros", [False, True])
+def test_linear_w4_large_finite_x(cuda, rows, n, k, group, zeros):
+    """x up to bf16's largest value: outputs are finite where their definition is."""
+    x, qw, s, z, b = w4_case(rows, n, k, group, zeros, True)
+    s = (s * 0.01).clamp(-6e-4, 6e-4)
+    top = torch.finfo(BF16).max
+    x[0, :group] = top                          # a whole group of one sign
+    x[rows // 2, 7], x[rows - 1, k - 1] = 1e37, -top
+    want, tol = w4_reference(x, qw, s, z, b)
+    assert (want.abs() < top).all()
+    close(K.linear_w4(x, qw, s, z, b), want, tol)
+
+
 def test_linear_w4_empty(cuda):
     x, qw, s, z, b = w4_case(3, 8, 64, 32, False, False)
     assert K.linear_w4(x[:0], qw, s).shape == (0, 8)
