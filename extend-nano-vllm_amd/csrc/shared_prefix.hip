@@ -541,7 +541,7 @@ void make_plan(PrefixParams& pp, int32_t prefix_len, int32_t block_size) {
   pp.prefix = prefix_len < p.max_k ? prefix_len / 32 * 32 : p.max_k / 32 * 32;
   p.qtile = kTileRows / p.group;
   pp.prefix_tiles = ceil_div(p.num_tokens, p.qtile);
-  pp.own_tiles = ceil_div(p.max_q, p.qtile);
+  pp.own_tiles = p.max_q > 0 ? ceil_div(p.max_q, p.qtile) : 1;   // one, which marks the rows past max_q
   const int64_t cus = device_cus();
   const float heads = static_cast<float>(p.num_tokens) * p.hq;
   const float units = static_cast<float>(pp.prefix_tiles) * p.hkv;   // of one part
@@ -602,7 +602,7 @@ int run(PrefixParams& pp, int kv_dtype, int32_t prefix_len, void* workspace, siz
   if (kv_dtype != NVA_KV_BF16 && kv_dtype != NVA_KV_FP8_E4M3) return NVA_ERR_ARG;
   if (p.num_seqs < 0 || p.num_tokens < 0 || p.max_q < 0 || p.max_k < 0 || prefix_len < 0) return NVA_ERR_ARG;
   if (!(p.scale_log2 > 0.0f)) return NVA_ERR_ARG;      // the running maximum is the scaled scores'
-  if (p.num_seqs == 0 || p.num_tokens == 0 || p.max_q == 0) return NVA_OK;
+  if (p.num_seqs == 0 || p.num_tokens == 0) return NVA_OK;
   if (!p.q || !p.k_cache || !p.v_cache || !p.block_tables || !p.out) return NVA_ERR_ARG;
   if (p.block_size <= 0 || p.block_size % 32 != 0 || p.num_blocks <= 0) return NVA_ERR_UNSUPPORTED;
   if (p.bt_cols < 0 || p.bt_stride < p.bt_cols) return NVA_ERR_ARG;
@@ -647,7 +647,7 @@ extern "C" size_t nva_shared_prefix_workspace_size(int32_t num_seqs, int32_t num
                                                    int32_t head_dim, int32_t max_seqlen_q,
                                                    int32_t max_seqlen_k, int32_t prefix_len) {
   if (num_seqs <= 0 || num_tokens <= 0 || num_q_heads <= 0 || num_kv_heads <= 0 || head_dim != kD ||
-      max_seqlen_q <= 0 || max_seqlen_k < 0 || prefix_len < 0 || num_q_heads % num_kv_heads ||
+      max_seqlen_q < 0 || max_seqlen_k < 0 || prefix_len < 0 || num_q_heads % num_kv_heads ||
       num_q_heads / num_kv_heads > 64)
     return 0;
   PrefixParams pp = {};

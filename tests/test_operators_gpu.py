@@ -661,6 +661,17 @@ def test_shared_prefix_values_that_are_not_finite_stay_with_the_rows_that_see_th
     close(got[~bad], want[~bad], tol[~bad])
 
 
+def test_shared_prefix_no_query_rows_within_the_bound(cuda):
+    """max_seqlen_q of 0 leaves every row of the batch past it: zeros, and rows of no
+    sequence as they were."""
+    rows, keys, prefix = [2, 1], [600, 540], 512
+    q, kc, vc, cu_q, cu_k, table = pages_case(rows, keys, prefix, 8, 4)
+    q = torch.cat([q, q[:2]])
+    out = torch.full((5, 8, D), 3.0, dtype=BF16, device="cuda")
+    K.shared_prefix_attention_varlen(q, kc, vc, cu_q, cu_k, 0, 600, prefix, SCALE, table, out=out)
+    assert (out[:3] == 0).all() and (out[3:] == 3).all()
+
+
 def test_shared_prefix_large_scores_and_stale_slots(cuda):
     # rows whose parts differ by hundreds in the exponent, infinities and NaN in
     # slots that no row sees
