@@ -555,6 +555,16 @@ PyObject* shared_prefix_attention_decode(PyObject*, PyObject* const* v, Py_ssize
   });
 }
 
+// Whether the address ranges of two tensors with elements are apart.
+bool apart(const at::Tensor& a, const at::Tensor& b) {
+  auto end = [](const at::Tensor& t) {
+    int64_t last = 0;
+    for (int64_t d = 0; d < t.dim(); ++d) last += (t.size(d) - 1) * t.stride(d);
+    return static_cast<char*>(t.data_ptr()) + (last + 1) * t.element_size();
+  };
+  return end(a) <= static_cast<char*>(b.data_ptr()) || end(b) <= static_cast<char*>(a.data_ptr());
+}
+
 bool wants_grad(const at::Tensor& t) { return at::GradMode::is_enabled() && t.requires_grad(); }
 
 // (x, qweight, scales, zeros | None, bias | None, out | None) -> out
@@ -594,6 +604,8 @@ PyObject* linear_w4(PyObject*, PyObject* const* v, Py_ssize_t n) {
       out = a.tensor(5);
       need_rows(out);
       need(out.size(0) == rows && out.size(1) == m && out.stride(0) >= m);
+      // inputs in out's range may still be other columns of its rows
+      for (int i = 0; i < 5; ++i) need(a.none(i) || apart(out, a.tensor(i)));
     }
     void* s = current_stream(a.device);
     const size_t bytes = nva_linear_w4_workspace_size(rows, m, k, group);

@@ -910,6 +910,10 @@ def linear_w4(x: torch.Tensor, qweight: torch.Tensor, scales: torch.Tensor,
         raise ValueError("out must be bf16 [rows, n] with unit last stride")
     if n == 0 or rows == 0:
         return out
+    # workgroups run in any order; x may be other columns of out's rows
+    if any(t is not None and _in_one_range(out, t) for t in (qweight, scales, zeros, bias)) \
+            or (_meet(out[:, None], x[:, None]) if x.stride(1) == 1 else _in_one_range(out, x)):
+        raise ValueError("out must not overlap the inputs")
     # the kernel reads x 16 bytes at a time, and rows of a slab within 2^31 bytes
     if x.stride(1) != 1 or (rows > 1 and (x.stride(0) % 8 or x.stride(0) < k)) \
             or (rows > 16 and x.stride(0) >= 1 << 24) or x.data_ptr() % 16:
@@ -928,6 +932,15 @@ def linear_w4(x: torch.Tensor, qweight: torch.Tensor, scales: torch.Tensor,
 
 _ROTARY_DTYPES = {BF16: _native.DTYPE_BF16, torch.float16: _native.DTYPE_F16,
                   torch.float32: _native.DTYPE_F32}
+
+
+def _in_one_range(a: torch.Tensor, b: torch.Tensor) -> bool:
+    """Whether the address ranges of two tensors with elements meet."""
+    lo, hi = [], []
+    for t in (a, b):
+        lo.append(t.data_ptr())
+        hi.append(lo[-1] + t.element_size() * (sum((n - 1) * s for n, s in zip(t.shape, t.stride())) + 1))
+    return lo[0] < hi[1] and lo[1] < hi[0]
 
 
 def _meet(a: torch.Tensor, b: torch.Tensor) -> bool:

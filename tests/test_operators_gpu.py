@@ -173,6 +173,30 @@ def test_linear_w4_large_finite_x(cuda, rows, n, k, group, zeros):
     close(K.linear_w4(x, qw, s, z, b), want, tol)
 
 
+def test_linear_w4_out_over_an_input_is_refused(cuda):
+    x, qw, s, z, b = w4_case(6, 128, 128, 64, True, True)
+    want = K.linear_w4(x, qw, s, z, b)
+    flat = torch.zeros(6 * 128 + 64, dtype=BF16, device="cuda")
+    moved = flat[:6 * 128].view(6, 128)
+    moved.copy_(x)
+    scales = torch.zeros(2 * 128 + 8, dtype=BF16, device="cuda")
+    scales[:2 * 128] = s.flatten()
+    held = scales[:2 * 128].view(2, 128)
+    codes = qw.clone()
+    for args, out in [((moved, qw, s, z, b), moved), ((moved, qw, s, z, b), flat[64:].view(6, 128)),
+                      ((x[:1], qw, held, z, b), scales[8:136].view(1, 128)),
+                      ((x, codes, s, z, b), codes.view(-1).view(BF16)[:6 * 128].view(6, 128)),
+                      ((x[:1], qw, s, z, held[0]), held[:1])]:
+        with pytest.raises(ValueError, match="overlap"):
+            K.linear_w4(*args, out=out)
+    assert torch.equal(moved, x)
+    # x and out as different columns of the same rows do not
+    both = torch.zeros(6, 272, dtype=BF16, device="cuda")
+    both[:, :128] = x
+    assert torch.equal(K.linear_w4(both[:, :128], qw, s, z, b, out=both[:, 136:264]), want)
+    assert torch.equal(both[:, :128], x) and (both[:, 128:136] == 0).all()
+
+
 def test_linear_w4_empty(cuda):
     x, qw, s, z, b = w4_case(3, 8, 64, 32, False, False)
     assert K.linear_w4(x[:0], qw, s).shape == (0, 8)
