@@ -484,6 +484,13 @@ PyObject* linear(PyObject*, PyObject* const* v, Py_ssize_t n) {
   });
 }
 
+bool wants_grad(const at::Tensor& t) { return at::GradMode::is_enabled() && t.requires_grad(); }
+
+// Attention over a shared prefix computes no gradients: q, the caches and the scales.
+void need_no_grad(const Args& a, int k_scale, int v_scale) {
+  for (int i : {0, 1, 2, k_scale, v_scale}) need(a.none(i) || !wants_grad(a.any(i)));
+}
+
 // (q, k_cache, v_cache, cu_q, cu_k, max_q, max_k, prefix_len, softmax_scale, block_table,
 //  k_scale | None, v_scale | None, out | None) -> out
 PyObject* shared_prefix_attention_varlen(PyObject*, PyObject* const* v, Py_ssize_t n) {
@@ -500,6 +507,7 @@ PyObject* shared_prefix_attention_varlen(PyObject*, PyObject* const* v, Py_ssize
     need_i32(cu_q);
     need_i32(cu_k);
     const int32_t b = as_i32(cu_q.numel() - 1);
+    need_no_grad(a, 10, 11);
     const Attention r = attention(a, q, 1, 2, bt, 12);
     need(b > 0 && cu_k.numel() == b + 1 && bt.size(0) >= b && r.t > 0 && r.hq > 0);
     need(prefix >= 0 && prefix <= int64_t{r.bt_cols} * r.p.block_size);
@@ -533,6 +541,7 @@ PyObject* shared_prefix_attention_decode(PyObject*, PyObject* const* v, Py_ssize
     const float* ks = a.scale(8);
     const float* vs = a.scale(9);
     need_i32(lens);
+    need_no_grad(a, 8, 9);
     const Attention r = attention(a, q, 1, 2, bt, 10);
     need(lens.numel() == r.t && bt.size(0) >= r.t && r.t > 0 && r.hq > 0);
     const int32_t all = as_i32(int64_t{r.bt_cols} * r.p.block_size);
@@ -564,8 +573,6 @@ bool apart(const at::Tensor& a, const at::Tensor& b) {
   };
   return end(a) <= static_cast<char*>(b.data_ptr()) || end(b) <= static_cast<char*>(a.data_ptr());
 }
-
-bool wants_grad(const at::Tensor& t) { return at::GradMode::is_enabled() && t.requires_grad(); }
 
 // (x, qweight, scales, zeros | None, bias | None, out | None) -> out
 PyObject* linear_w4(PyObject*, PyObject* const* v, Py_ssize_t n) {

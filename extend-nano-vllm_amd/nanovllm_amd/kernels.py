@@ -575,6 +575,7 @@ def shared_prefix_attention_varlen(q: torch.Tensor, k_cache: torch.Tensor, v_cac
         return got
     lib = _native.load()
     _require_cuda(q, k_cache, v_cache, block_table, out, _scale(k_scale), _scale(v_scale))
+    _no_grad("shared_prefix_attention", q, k_cache, v_cache, k_scale, v_scale)
     cu_seqlens_q, host_q = _device_lengths(cu_seqlens_q, q.device, "cu_seqlens_q")
     cu_seqlens_k, host_k = _device_lengths(cu_seqlens_k, q.device, "cu_seqlens_k")
     if host_q is not None:
@@ -623,6 +624,7 @@ def shared_prefix_attention_decode(q: torch.Tensor, k_cache: torch.Tensor, v_cac
         return got
     lib = _native.load()
     _require_cuda(q, k_cache, v_cache, block_table, out, _scale(k_scale), _scale(v_scale))
+    _no_grad("shared_prefix_attention", q, k_cache, v_cache, k_scale, v_scale)
     cache_seqlens, host_lens = _device_lengths(cache_seqlens, q.device, "cache_seqlens")
     _i32(cache_seqlens, "cache_seqlens")
     b = q.shape[0]

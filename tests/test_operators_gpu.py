@@ -764,6 +764,25 @@ def test_shared_prefix_refusals(cuda):
             call(**kw)
 
 
+def test_shared_prefix_refuses_gradients(cuda):
+    rows, keys, prefix = [1, 1], [600, 540], 512
+    q, kc, vc, cu_q, cu_k, table = pages_case(rows, keys, prefix, 8, 4)
+    lens = torch.tensor(keys, dtype=torch.int32, device="cuda")
+    one = torch.ones(1, device="cuda")
+    want = K.shared_prefix_attention_decode(q, kc, vc, lens, table, prefix, SCALE)
+    wants = lambda t: t.detach().requires_grad_()  # noqa: E731
+    for a, kw in (((wants(q), kc, vc), {}), ((q, wants(kc), vc), {}), ((q, kc, wants(vc)), {}),
+                  ((q, kc, vc), dict(k_scale=wants(one), v_scale=one)),
+                  ((q, kc, vc), dict(k_scale=one, v_scale=wants(one)))):
+        with pytest.raises(ValueError, match="gradients"):
+            K.shared_prefix_attention_decode(*a, lens, table, prefix, SCALE, **kw)
+        with pytest.raises(ValueError, match="gradients"):
+            K.shared_prefix_attention_varlen(*a, cu_q, cu_k, 1, 600, prefix, SCALE, table, **kw)
+        with torch.no_grad():
+            assert torch.equal(K.shared_prefix_attention_decode(*a, lens, table, prefix, SCALE, **kw),
+                               want)
+
+
 # ---------------------------------------------------------------- streams, graphs, a step
 
 def step_state(seed=0, batch=6, hidden=512, hq=8, hkv=2, prefix=512):
