@@ -491,6 +491,16 @@ void need_no_grad(const Args& a, int k_scale, int v_scale) {
   for (int i : {0, 1, 2, k_scale, v_scale}) need(a.none(i) || !wants_grad(a.any(i)));
 }
 
+// [rows, heads, d] whose heads do not overlap: heads within rows, or rows within heads.
+void need_apart(const at::Tensor& t) {
+  auto nested = [&](int outer, int inner) {
+    const int64_t d = t.size(2), s = t.stride(inner);
+    return (t.size(inner) == 1 || s >= d) &&
+           (t.size(outer) == 1 || t.stride(outer) >= (t.size(inner) - 1) * s + d);
+  };
+  need(nested(0, 1) || nested(1, 0));
+}
+
 // (q, k_cache, v_cache, cu_q, cu_k, max_q, max_k, prefix_len, softmax_scale, block_table,
 //  k_scale | None, v_scale | None, out | None) -> out
 PyObject* shared_prefix_attention_varlen(PyObject*, PyObject* const* v, Py_ssize_t n) {
@@ -509,6 +519,7 @@ PyObject* shared_prefix_attention_varlen(PyObject*, PyObject* const* v, Py_ssize
     const int32_t b = as_i32(cu_q.numel() - 1);
     need_no_grad(a, 10, 11);
     const Attention r = attention(a, q, 1, 2, bt, 12);
+    need_apart(r.out);
     need(b > 0 && cu_k.numel() == b + 1 && bt.size(0) >= b && r.t > 0 && r.hq > 0);
     need(prefix >= 0 && prefix <= int64_t{r.bt_cols} * r.p.block_size);
     void* s = current_stream(a.device);
@@ -543,6 +554,7 @@ PyObject* shared_prefix_attention_decode(PyObject*, PyObject* const* v, Py_ssize
     need_i32(lens);
     need_no_grad(a, 8, 9);
     const Attention r = attention(a, q, 1, 2, bt, 10);
+    need_apart(r.out);
     need(lens.numel() == r.t && bt.size(0) >= r.t && r.t > 0 && r.hq > 0);
     const int32_t all = as_i32(int64_t{r.bt_cols} * r.p.block_size);
     const int32_t max_k = a.none(7) ? all : a.i32(7);

@@ -548,7 +548,10 @@ def _prefix_args(q, k_cache, v_cache, block_table, num_seqs: int, prefix_len: in
         raise ValueError("max_seqlen_k must not be negative")
     if not scale > 0:
         raise ValueError("softmax_scale must be positive")
-    return cache, _q_out(q, out)
+    out = _q_out(q, out)
+    if _self_overlap(out):
+        raise ValueError("out must not overlap itself")
+    return cache, out
 
 
 def shared_prefix_attention_varlen(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor,

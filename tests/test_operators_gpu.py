@@ -783,6 +783,25 @@ def test_shared_prefix_refuses_gradients(cuda):
                                want)
 
 
+def test_shared_prefix_out_that_overlaps_itself_is_refused(cuda):
+    rows, keys, prefix = [1, 1, 1], [600, 540, 513], 512
+    q, kc, vc, cu_q, cu_k, table = pages_case(rows, keys, prefix, 8, 4)
+    lens = torch.tensor(keys, dtype=torch.int32, device="cuda")
+    want = K.shared_prefix_attention_decode(q, kc, vc, lens, table, prefix, SCALE)
+    flat = torch.zeros(3 * 8 * D, dtype=BF16, device="cuda")
+    for strides in ((0, D, 1), (8 * D, 0, 1), (D, D, 1), (4 * D, D, 1), (8 * D, 64, 1)):
+        out = flat.as_strided((3, 8, D), strides)
+        with pytest.raises(ValueError, match="overlap"):
+            K.shared_prefix_attention_decode(q, kc, vc, lens, table, prefix, SCALE, out=out)
+        with pytest.raises(ValueError, match="overlap"):
+            K.shared_prefix_attention_varlen(q, kc, vc, cu_q, cu_k, 1, 600, prefix, SCALE, table, out=out)
+    assert (flat == 0).all()
+    for out in (torch.zeros(8, 3, D, dtype=BF16, device="cuda").transpose(0, 1),
+                torch.zeros(3, 8, 2 * D, dtype=BF16, device="cuda")[..., D:]):
+        K.shared_prefix_attention_decode(q, kc, vc, lens, table, prefix, SCALE, out=out)
+        assert torch.equal(out, want)
+
+
 # ---------------------------------------------------------------- streams, graphs, a step
 
 def step_state(seed=0, batch=6, hidden=512, hq=8, hkv=2, prefix=512):
