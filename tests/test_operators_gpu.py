@@ -696,6 +696,42 @@ def test_shared_prefix_no_query_rows_within_the_bound(cuda):
     assert (out[:3] == 0).all() and (out[3:] == 3).all()
 
 
+def clipped_lengths(rows, keys, max_q, max_k):
+    """What a call with these bounds computes: (rows, keys) of every sequence."""
+    kept = [min(r, max_q) for r in rows]
+    return kept, [min(n - (r - a), max_k) for r, a, n in zip(rows, kept, keys)]
+
+
+@pytest.mark.parametrize("fp8", [False, True])
+@pytest.mark.parametrize("mq,mk", [(4, 900), (6, 899), (6, 700), (6, 699), (6, 559), (3, 512), (5, 511),
+                                   (2, 100), (1, 33), (6, 1)])
+def test_shared_prefix_clips_to_the_bounds(cuda, mq, mk, fp8):
+    """Against the definition on the clipped lengths, where the first key that a
+    bound cuts off would take all the weight."""
+    rows, keys, prefix = [6, 2, 4], [900, 700, 560], 512
+    q, kc, vc, cu_q, cu_k, table = pages_case(rows, keys, prefix, 8, 4, fp8=fp8)
+    kept, seen = clipped_lengths(rows, keys, mq, mk)
+    starts = [0, 6, 8]
+    planted = [i for i, n in enumerate(seen) if n < keys[i] and (n >= prefix or (n == max(seen) and i == 0))]
+    for i in planted:       # the key behind the last one that the sequence sees
+        page, at = int(table[i, seen[i] // 256]), seen[i] % 256
+        row = q[starts[i] + kept[i] - 1].view(4, 2, D)[:, 0].float() * 4
+        kc[page, at], vc[page, at] = row.to(kc.dtype), torch.full_like(row, 400.0).to(vc.dtype)
+    assert planted
+    first = torch.cat([torch.arange(s, s + r) for s, r in zip(starts, kept)])
+    want, tol = (torch.zeros(q.shape, dtype=torch.float64) for _ in range(2))
+    want[first], tol[first] = prefix_reference(q[first.cuda()], kc, vc, kept, seen, table, SCALE)
+    over, _ = prefix_reference(q[first.cuda()], kc, vc, kept,
+                               [n + (i in planted) for i, n in enumerate(seen)], table, SCALE)
+    ends = torch.tensor(kept).cumsum(0) - 1
+    for i in planted:       # seen all the same, it would show
+        assert ((over - want[first]).abs() > 100 * tol[first])[ends[i]].any()
+    one = torch.ones(1, device="cuda")
+    got = K.shared_prefix_attention_varlen(q, kc, vc, cu_q, cu_k, mq, mk, prefix, SCALE, table,
+                                           k_scale=one, v_scale=one)
+    close(got, want, tol)
+
+
 def test_shared_prefix_large_scores_and_stale_slots(cuda):
     # rows whose parts differ by hundreds in the exponent, infinities and NaN in
     # slots that no row sees
