@@ -89,6 +89,18 @@ def rope_cos_sin(head_dim: int, max_position: int, base: float, device_index: in
     return table.to(torch.device("cuda", device_index))
 
 
+# The keys of a rope_scaling dict that rope_frequencies reads, by type.
+_ROPE_KEYS = {
+    "default": (),
+    "linear": ("factor",),
+    "dynamic": ("factor",),
+    "yarn": ("factor", "beta_fast", "beta_slow", "truncate", "attention_factor", "mscale",
+             "mscale_all_dim"),
+    "llama3": ("factor", "low_freq_factor", "high_freq_factor"),
+    "longrope": ("factor", "short_factor", "long_factor", "attention_factor"),
+}
+
+
 def rope_frequencies(rotary_dim: int, base: float, scaling: dict | None = None,
                      max_position: int | None = None, seq_len: int | None = None):
     """(inv_freq, factor) of ``kernels.rotary_embedding``: float64 angles per
@@ -105,18 +117,34 @@ def rope_frequencies(rotary_dim: int, base: float, scaling: dict | None = None,
       sequence of n = ``seq_len`` > o tokens, d = rotary_dim;
     * "yarn": f_i / s where f_i turns at most beta_slow (1) times over o
       positions, f_i where it turns at least beta_fast (32) times, with a linear
-      ramp over i between; factor 0.1 ln s + 1 unless "attention_factor" says;
+      ramp over i between, whose ends are whole pairs unless "truncate" is false;
+      factor "attention_factor" if given, else m(mscale) / m(mscale_all_dim) if
+      both are, else m(1), with m(a) = 0.1 a ln s + 1 for s > 1 and 1 otherwise;
     * "llama3": f_i / s for wavelengths past o / low_freq_factor, f_i below
       o / high_freq_factor, interpolated in o / wavelength between;
     * "longrope": f_i / c_i with c the "long_factor" list where seq_len > o, else
       "short_factor"; factor sqrt(1 + ln s / ln o) for s > 1, s = max_position / o
-      unless given, unless "attention_factor" says."""
+      unless given, unless "attention_factor" says.
+
+    Keys that the type does not read (None counts as absent) raise ValueError: they
+    would change the positions of the model they come with.  "rope_theta" has to be
+    ``base``; "partial_rotary_factor" is in rotary_dim, and "finetuned" says nothing
+    about the frequencies."""
     if rotary_dim <= 0 or rotary_dim % 2:
         raise ValueError("rotary_dim must be a positive even number")
     i = torch.arange(rotary_dim // 2, dtype=torch.float64, device="cpu")
     freq = float(base) ** (-2.0 * i / rotary_dim)
     scaling = dict(scaling or {})
     kind = scaling.get("rope_type", scaling.get("type", "default"))
+    if kind not in _ROPE_KEYS:
+        raise ValueError(f"unknown rope_scaling type: {kind!r}")
+    known = ("rope_type", "type", "original_max_position_embeddings", "rope_theta",
+             "partial_rotary_factor", "finetuned", *_ROPE_KEYS[kind])
+    extra = sorted(k for k, v in scaling.items() if v is not None and k not in known)
+    if extra:
+        raise ValueError(f"rope_scaling of type {kind!r} with keys that are not read: {extra}")
+    if scaling.get("rope_theta") is not None and float(scaling["rope_theta"]) != float(base):
+        raise ValueError("rope_scaling's rope_theta is not the base")
     if kind == "default":
         return freq, 1.0
     trained = scaling.get("original_max_position_embeddings") or max_position
@@ -143,12 +171,22 @@ def rope_frequencies(rotary_dim: int, base: float, scaling: dict | None = None,
         def pair_of(turns):     # the (fractional) pair that turns so often over the trained positions
             return rotary_dim * math.log(trained / (turns * 2 * math.pi)) / (2 * math.log(base))
 
-        low = max(math.floor(pair_of(float(scaling.get("beta_fast") or 32))), 0)
-        high = min(math.ceil(pair_of(float(scaling.get("beta_slow") or 1))), rotary_dim - 1)
+        def amplitude(a):
+            return 0.1 * a * math.log(s) + 1.0 if s > 1 else 1.0
+
+        low = pair_of(float(scaling.get("beta_fast") or 32))
+        high = pair_of(float(scaling.get("beta_slow") or 1))
+        if scaling.get("truncate") in (None, True):
+            low, high = math.floor(low), math.ceil(high)
+        low, high = max(low, 0), min(high, rotary_dim - 1)
         ramp = ((i - low) / max(high - low, 0.001)).clamp(0.0, 1.0)
+        scales = [scaling.get(k) for k in ("mscale", "mscale_all_dim")]
         factor = scaling.get("attention_factor")
         if factor is None:
-            factor = 0.1 * math.log(s) + 1.0 if s > 1 else 1.0
+            if (scales[0] is None) != (scales[1] is None):
+                raise ValueError("rope_scaling of type 'yarn' needs mscale and mscale_all_dim, or neither")
+            factor = amplitude(1.0) if scales[0] is None else \
+                amplitude(float(scales[0])) / amplitude(float(scales[1]))
         return freq / s * ramp + freq * (1.0 - ramp), float(factor)
     if kind == "llama3":
         s = float(value("factor"))
@@ -166,7 +204,6 @@ def rope_frequencies(rotary_dim: int, base: float, scaling: dict | None = None,
             s = scaling.get("factor") or (max_position or trained) / trained
             factor = math.sqrt(1.0 + math.log(s) / math.log(trained)) if s > 1 else 1.0
         return freq / c, float(factor)
-    raise ValueError(f"unknown rope_scaling type: {kind!r}")
 
 
 class Attention(nn.Module):

@@ -88,6 +88,60 @@ def test_frequencies_yarn():
     assert factor == 1.5 and torch.equal(given, got)
 
 
+def test_frequencies_yarn_amplitude():
+    def factor(s=40.0, **kw):
+        return rope_frequencies(64, 1e4, dict(type="yarn", factor=s, original_max_position_embeddings=4096,
+                                              **kw))[1]
+
+    m = 0.1 * math.log(40)
+    assert math.isclose(factor(), m + 1)
+    assert factor(mscale=1.0, mscale_all_dim=1.0) == 1.0
+    assert math.isclose(factor(mscale=0.707, mscale_all_dim=1.0), (0.707 * m + 1) / (m + 1))
+    assert math.isclose(factor(mscale=1.0, mscale_all_dim=0.0), m + 1)
+    assert factor(mscale=2.0, mscale_all_dim=0.5, attention_factor=1.25) == 1.25
+    assert factor(s=1.0, mscale=2.0, mscale_all_dim=0.5) == 1.0
+    for kw in (dict(mscale=0.707), dict(mscale_all_dim=1.0)):
+        with pytest.raises(ValueError, match="mscale"):
+            factor(**kw)
+
+
+def test_frequencies_yarn_ends_of_the_ramp():
+    """factor 8, 4096 positions, base 1e4, 64 elements: the pair that turns 32 times is
+    64 ln(4096 / (64 pi)) / (2 ln 1e4) = 10.47, the one that turns once 22.51."""
+    scaling = dict(type="yarn", factor=8.0, original_max_position_embeddings=4096)
+    freq, _ = rope_frequencies(64, 1e4)
+    low, high = (64 * math.log(4096 / (t * 2 * math.pi)) / (2 * math.log(1e4)) for t in (32, 1))
+    assert 10.4 < low < 10.5 and 22.5 < high < 22.6
+    for truncate, a, b in ((None, 10, 23), (True, 10, 23), (False, low, high)):
+        got, factor = rope_frequencies(64, 1e4, dict(scaling, truncate=truncate))
+        assert math.isclose(factor, 0.1 * math.log(8) + 1)
+        for i in range(32):
+            ramp = min(max((i - a) / (b - a), 0.0), 1.0)
+            want = float(freq[i]) * ((1 - ramp) + ramp / 8)
+            assert math.isclose(float(got[i]), want, rel_tol=1e-12), (truncate, i)
+
+
+def test_frequencies_refuse_keys_they_do_not_read():
+    base = {"default": {}, "linear": dict(factor=2.0), "dynamic": dict(factor=2.0),
+            "yarn": dict(factor=2.0), "llama3": dict(factor=8.0, low_freq_factor=1.0, high_freq_factor=4.0),
+            "longrope": dict(short_factor=[1.0] * 32, long_factor=[2.0] * 32)}
+    for kind, keys in base.items():
+        scaling = dict(rope_type=kind, original_max_position_embeddings=4096, **keys)
+        want = rope_frequencies(64, 1e4, scaling, seq_len=8192)
+        kept = dict(scaling, rope_theta=1e4, partial_rotary_factor=0.5, finetuned=True, attn_factor=None)
+        got = rope_frequencies(64, 1e4, kept, seq_len=8192)
+        assert torch.equal(got[0], want[0]) and got[1] == want[1]
+        for extra in (dict(attn_factor=2.0), dict(short_mscale=1.2), dict(mrope_section=[8, 12, 12]),
+                      dict(extrapolation_factor=1.0), dict(alpha=2.0)):
+            with pytest.raises(ValueError, match="not read"):
+                rope_frequencies(64, 1e4, dict(scaling, **extra), seq_len=8192)
+        if kind != "yarn":
+            with pytest.raises(ValueError, match="not read"):
+                rope_frequencies(64, 1e4, dict(scaling, truncate=False), seq_len=8192)
+        with pytest.raises(ValueError, match="rope_theta"):
+            rope_frequencies(64, 1e4, dict(scaling, rope_theta=5e5), seq_len=8192)
+
+
 def test_frequencies_llama3():
     scaling = dict(rope_type="llama3", factor=8.0, low_freq_factor=1.0, high_freq_factor=4.0,
                    original_max_position_embeddings=8192)
