@@ -845,8 +845,8 @@ def quantize_w4(weight: torch.Tensor, group_size: int = 128, zeros: bool = False
     [k / group_size, n] or None).
 
     Rounds each weight to the nearest of 16 levels of its group: without zeros
-    -8 .. 7 times the scale, the largest magnitude at 7 or at -8, whichever
-    leaves the smaller scale; with zeros from the group's least value (or 0) to
+    -8 .. 7 times the scale, which is the least that holds both ends (a group
+    from -8 to 8 has 8 / 7); with zeros from the group's least value (or 0) to
     its greatest (or 0).  Scales are rounded to bf16 before the codes are
     formed, so the codes are the nearest for the scale that is used."""
     if weight.dim() != 2 or not weight.is_floating_point():

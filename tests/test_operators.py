@@ -53,6 +53,16 @@ def test_quantize_w4_keeps_what_four_bits_hold():
     assert z is None and torch.equal(dequantized(qw, s, z)[0], w)
 
 
+@pytest.mark.parametrize("lo,hi,scale", [(-8.0, 8.0, 8 / 7), (-8.0, 3.0, 1.0), (-3.0, 7.0, 1.0),
+                                         (1.0, 14.0, 2.0), (-16.0, -1.0, 2.0)])
+def test_quantize_w4_takes_the_least_scale_that_holds_both_ends(lo, hi, scale):
+    w = torch.linspace(lo, hi, 64)[None]
+    qw, s, _ = K.quantize_w4(w, 64)
+    assert float(s) == float(torch.tensor(scale).to(BF16))
+    back, step = dequantized(qw, s, None)
+    assert ((back - w.double()).abs() <= (0.5 + 8 * 2.0 ** -8) * step).all()   # 8 steps of the scale's rounding
+
+
 def test_quantize_w4_refusals():
     w = torch.zeros(4, 128)
     for args in [(w, 16), (w, 96), (w, 0), (w, -32), (w[0], 32), (w.int(), 32), (w[:, :0], 32)]:
