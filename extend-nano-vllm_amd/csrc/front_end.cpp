@@ -66,10 +66,10 @@ struct Args {
     if (!PyFloat_CheckExact(v[i])) throw Other{};
     return static_cast<float>(PyFloat_AS_DOUBLE(v[i]));
   }
-  // one-element float32 tensor or None
-  const float* scale(int i) const {
+  // one-element float32 tensor on the others' device, or None
+  const float* scale(int i) {
     if (none(i)) return nullptr;
-    const at::Tensor& t = any(i);
+    const at::Tensor& t = tensor(i);
     need(t.scalar_type() == at::kFloat && t.numel() == 1);
     return static_cast<const float*>(t.data_ptr());
   }

@@ -819,6 +819,16 @@ def test_shared_prefix_refuses_gradients(cuda):
                                want)
 
 
+@pytest.mark.skipif(torch.cuda.device_count() < 2, reason="needs two GPUs")
+def test_shared_prefix_scales_on_another_device_are_refused(cuda):
+    q, kc, vc, _, _, table = pages_case([1, 1], [600, 540], 512, 8, 4, fp8=True)
+    lens = torch.tensor([600, 540], dtype=torch.int32, device="cuda")
+    one, far = torch.ones(1, device="cuda"), torch.ones(1, device="cuda:1")
+    for kw in (dict(k_scale=far, v_scale=one), dict(k_scale=one, v_scale=far)):
+        with pytest.raises(ValueError, match="same device"):
+            K.shared_prefix_attention_decode(q, kc, vc, lens, table, 512, SCALE, **kw)
+
+
 def test_shared_prefix_out_that_overlaps_itself_is_refused(cuda):
     rows, keys, prefix = [1, 1, 1], [600, 540, 513], 512
     q, kc, vc, cu_q, cu_k, table = pages_case(rows, keys, prefix, 8, 4)
