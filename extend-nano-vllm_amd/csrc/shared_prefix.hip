@@ -530,7 +530,11 @@ int own_kind(int64_t rows) { return rows <= 16 ? 1 : rows <= 32 ? 2 : rows <= 64
 // row and head at 3.5 TB/s) and the units' start (5 us over 512 places), where a
 // part costs three times that beside the own keys' units.  Past a unit a CU, as
 // many as fill one or two a CU.  Own keys are cut into parts of about 512 keys, 320
-// where there are few units.  Over 16 shapes (batches of 2-160, 1-64 rows, heads
+// where there are few units; prompts (several tiles a sequence) no further than two
+// rounds of units, since every part is a slot of every row: 8 x 2048 rows of 64/8
+// heads over 4096 + 4096 keys take 1.1 GB of workspace and 4.53 ms (parts of 512: 4.9 GB,
+// 5.88 ms), 1 x 4096 rows over 36864 own keys 0.27 GB and 5.6 ms (9.9 GB, 9.0 ms), 4 x
+// 512 rows over 4096 + 512 at 32/8 182 us (179).  Over 16 shapes (batches of 2-160, 1-64 rows, heads
 // 5/1-64/8, prefixes of 512-16384 keys, bf16 and FP8) timed with all counts of
 // parts the choice is 3% from the best on the geometric mean; a part more or
 // less around it costs little: 64 x 8192 shared keys at 32/8 heads 4 / 6 / 8 / 12 /
@@ -561,11 +565,15 @@ void make_plan(PrefixParams& pp, int32_t prefix_len, int32_t block_size) {
   // own keys
   const int32_t own = p.max_k - pp.prefix;
   const int32_t length = static_cast<int64_t>(p.num_seqs) * pp.own_tiles * p.hkv < cus / 2 ? 320 : 512;
-  const int32_t own_count = own / length + (own % length >= length / 2 ? 1 : 0);
+  int32_t own_count = own / length + (own % length >= length / 2 ? 1 : 0);
+  if (pp.own_tiles > 1) {
+    const int64_t rounds = 4 * cus / (static_cast<int64_t>(pp.prefix_tiles) * p.hkv);
+    if (own_count > rounds) own_count = static_cast<int32_t>(rounds);
+  }
   pp.own_split = own > 0 ? ceil_div(ceil_div(own, own_count < 1 ? 1 : own_count), kWideKeys) * kWideKeys : kWideKeys;
-  // attend_segment holds a part's block ids one a lane
+  // attend_segment and attend_tile hold a part's block ids one a lane
   const int32_t span = (kWave - 2) * (block_size > 0 ? block_size : kChunk) / kWideKeys * kWideKeys;
-  if (pp.own_split > span) pp.own_split = span;
+  if (own_kind(static_cast<int64_t>(p.max_q) * p.group) < 4 && pp.own_split > span) pp.own_split = span;
   pp.own_parts = own > 0 ? ceil_div(own, pp.own_split) : 1;
   p.max_splits = pp.prefix_parts + pp.own_parts;
   const int64_t prefix_units = static_cast<int64_t>(pp.prefix_parts) * pp.prefix_tiles;

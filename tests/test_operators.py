@@ -268,6 +268,17 @@ def test_prefix_workspace_holds_every_part():
         assert size(*bad) == 0
 
 
+@pytest.mark.parametrize("seqs,t,hq,hkv,mq,mk,prefix,parts", [
+    (8, 16384, 64, 8, 2048, 8192, 4096, 2), (1, 4096, 64, 8, 4096, 40960, 4096, 2),
+    (1, 4096, 64, 8, 4096, 40960, 36864, 3), (2, 2000, 16, 2, 1000, 31024, 1024, 10),
+    (4, 8192, 32, 8, 2048, 2048, 0, 1)])
+def test_prefix_workspace_of_prompts_stays_with_few_parts(seqs, t, hq, hkv, mq, mk, prefix, parts):
+    """A part costs 516 bytes a row and head: rows that fill the device by themselves
+    are not split as far as a decode batch's."""
+    size = _native.load().nva_shared_prefix_workspace_size(seqs, t, hq, hkv, 128, mq, mk, prefix)
+    assert size <= t * (hq * parts * 129 * 4 + 4)
+
+
 def test_tensors_on_the_host_are_refused():
     x = torch.zeros(2, 64, dtype=BF16)
     with pytest.raises(ValueError, match="device"):

@@ -537,6 +537,19 @@ def test_shared_prefix(cuda, name, fp8):
 
 
 @pytest.mark.parametrize("fp8", [False, True])
+@pytest.mark.parametrize("block", [32, 256])
+def test_shared_prefix_prompts_whose_keys_stay_in_one_part(cuda, block, fp8):
+    # more keys a part than a wave's lanes hold small pages
+    rows, keys, prefix = [1500, 548, 3], [3300, 2900, 2600], 224
+    q, kc, vc, cu_q, cu_k, table = pages_case(rows, keys, prefix, 64, 8, block=block, fp8=fp8)
+    want, tol = prefix_reference(q, kc, vc, rows, keys, table, SCALE)
+    one = torch.ones(1, device="cuda")
+    got = K.shared_prefix_attention_varlen(q, kc, vc, cu_q, cu_k, 1500, 3300, prefix, SCALE, table,
+                                           k_scale=one, v_scale=one)
+    close(got, want, tol)
+
+
+@pytest.mark.parametrize("fp8", [False, True])
 def test_shared_prefix_layouts(cuda, fp8):
     rows, keys, prefix = [2, 5, 1], [900, 600, 512], 512
     q, kc, vc, cu_q, cu_k, table = pages_case(rows, keys, prefix, 16, 4, fp8=fp8, token_major=True)
