@@ -82,21 +82,20 @@ template <typename T, int N>
 struct alignas(sizeof(T) * N < 16 ? sizeof(T) * N : 16) Pack {
   T v[N];
 };
-// two elements wherever they lie
+// two of them, aligned as one
 template <typename T>
 struct Two {
   T v[2];
 };
 
 // P: pairs of a unit.  Half layout: P elements at i and P at i + pairs;
-// interleaved: 2 P elements side by side.  A tail unit copies 2 P elements in
-// accesses of the pairs' size; units of one pair take any address, and the last
-// of an odd tail copies one element.
+// interleaved: 2 P elements side by side.  A tail unit copies 2 P elements, at
+// the pairs' alignment; units of one pair take any address, and the last of an
+// odd tail copies one element.
 template <typename T, int P, bool INTERLEAVED>
 __global__ void __launch_bounds__(kThreads) rotary_kernel(RotaryParams p) {
   using Unit = std::conditional_t<P == 1, Two<T>, Pack<T, 2 * P>>;   // of the interleaved layout
-  using Piece = std::conditional_t<INTERLEAVED && P != 1, Unit, Pack<T, P>>;
-  constexpr int kPiece = sizeof(Piece) / sizeof(T);
+  using Tail = std::conditional_t<INTERLEAVED, Unit, Two<Pack<T, P>>>;
   __shared__ float2 turn[kMaxPairs];
   const int64_t t = blockIdx.x;
   const double position = static_cast<double>(p.positions[t]);
@@ -114,10 +113,12 @@ __global__ void __launch_bounds__(kThreads) rotary_kernel(RotaryParams p) {
     T* out = static_cast<T*>(hd.out) + t * hd.out_row + h * hd.out_head;
     if (c >= p.pair_chunks) {
       const int d = 2 * p.pairs + 2 * P * (c - p.pair_chunks);
-#pragma unroll
-      for (int e = 0; e < 2 * P; e += kPiece)
-        if (P > 1 || e == 0 || d + e < p.head_dim)
-          *reinterpret_cast<Piece*>(out + d + e) = *reinterpret_cast<const Piece*>(in + d + e);
+      if constexpr (P > 1) {
+        *reinterpret_cast<Tail*>(out + d) = *reinterpret_cast<const Tail*>(in + d);
+      } else {
+        out[d] = in[d];
+        if (d + 1 < p.head_dim) out[d + 1] = in[d + 1];
+      }
       continue;
     }
     const float2* cs = turn + P * c;
