@@ -29,6 +29,7 @@ namespace {
 constexpr int kWaves = 4;
 constexpr int kThreads = kWave * kWaves;
 constexpr int kTileRows = 32 * kWaves;               // query rows of a wide tile
+constexpr int32_t kMaxKeys = 1 << 30;                // ends of parts are rounded up in 32 bits
 constexpr int kParkPitch = kD + 4;                   // floats per row of a part on its way out
 constexpr int kSegDwords = 2 * kWaves * kVStage;     // attend_segment's stages, then its query operands
 constexpr int kWideDwords = 2 * kWideBuf;
@@ -615,7 +616,7 @@ int run(PrefixParams& pp, int kv_dtype, int32_t prefix_len, void* workspace, siz
   if (p.block_size <= 0 || p.block_size % 32 != 0 || p.num_blocks <= 0) return NVA_ERR_UNSUPPORTED;
   if (p.bt_cols < 0 || p.bt_stride < p.bt_cols) return NVA_ERR_ARG;
   p.group = p.hq / p.hkv;
-  if (p.group > 64) return NVA_ERR_UNSUPPORTED;
+  if (p.group > 64 || p.max_k > kMaxKeys) return NVA_ERR_UNSUPPORTED;
   const int64_t vec = kv_dtype == NVA_KV_BF16 ? 8 : 16;        // elements of a 16-byte access
   if (!aligned16(p.q) || !aligned16(p.out) || !aligned16(p.k_cache) || !aligned16(p.v_cache) ||
       p.q_row_stride % 8 || p.q_head_stride % 8 || p.out_row_stride % 8 || p.out_head_stride % 8 ||
@@ -655,7 +656,7 @@ extern "C" size_t nva_shared_prefix_workspace_size(int32_t num_seqs, int32_t num
                                                    int32_t head_dim, int32_t max_seqlen_q,
                                                    int32_t max_seqlen_k, int32_t prefix_len) {
   if (num_seqs <= 0 || num_tokens <= 0 || num_q_heads <= 0 || num_kv_heads <= 0 || head_dim != kD ||
-      max_seqlen_q < 0 || max_seqlen_k < 0 || prefix_len < 0 || num_q_heads % num_kv_heads ||
+      max_seqlen_q < 0 || max_seqlen_k < 0 || max_seqlen_k > kMaxKeys || prefix_len < 0 || num_q_heads % num_kv_heads ||
       num_q_heads / num_kv_heads > 64)
     return 0;
   PrefixParams pp = {};

@@ -538,14 +538,16 @@ int nva_rotary_embedding(const int64_t *positions, const double *inv_freq, float
  *   prefix_len >= 0; the part beyond its last multiple of 32 keys is read
  *   through each sequence's own row.  Everything else as for K1: strides,
  *   dtypes, scales, the clip by max_seqlen_q / max_seqlen_k (which count the
- *   prefix), block ids outside the cache.  Rows of no sequence are not written.
+ *   prefix; max_seqlen_k <= 2^30), block ids outside the cache.  Rows of no sequence are not written.
  *   An infinity or NaN in V of a prefix key stays with the rows that see the
  *   key; in V of one of a sequence's other keys it may reach rows of that
  *   sequence that stand before the key, as in K1.
  *   While the prefix's bytes, counted once a sequence, stay below about 128 MiB
  *   (32 MiB in FP8), nva_paged_attention_* is the faster call.
  * workspace: nva_shared_prefix_workspace_size(...) bytes, 16-byte aligned, no
- *   initialisation; sized for the call's own shape.
+ *   initialisation; sized for the call's own shape.  516 bytes for every part of
+ *   every row and head: 1.1 GB for 8 x 2048 rows of 64 heads over 8192 keys (the
+ *   paged attention needs none there).
  * ------------------------------------------------------------------- */
 size_t nva_shared_prefix_workspace_size(int32_t num_seqs, int32_t num_tokens, int32_t num_q_heads,
                                         int32_t num_kv_heads, int32_t head_dim,

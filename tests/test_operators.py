@@ -279,6 +279,19 @@ def test_prefix_workspace_of_prompts_stays_with_few_parts(seqs, t, hq, hkv, mq, 
     assert size <= t * (hq * parts * 129 * 4 + 4)
 
 
+def test_prefix_attention_bounds_past_2_to_the_30_keys_are_refused():
+    lib = _native.load()
+    size = lib.nva_shared_prefix_workspace_size
+    for max_k in ((1 << 30) + 1, 2 ** 31 - 64, 2 ** 31 - 1):
+        assert size(8, 16384, 64, 8, 128, 2048, max_k, 4096) == 0
+        assert lib.nva_shared_prefix_attention_varlen(
+            P, 64 * 128, 128, P, P, 0, 256 * 128, 128, 256 * 128, 8, 256, P, P, P, 4, 4, 8, 16384,
+            2048, max_k, 512, 64, 8, 128, 0.1, None, None, P, 64 * 128, 128, P, 1 << 40,
+            None) == _native.NVA_ERR_UNSUPPORTED
+    # the largest bound is planned without coming round: a slot for every row and head
+    assert 16384 * 64 * 516 <= size(8, 16384, 64, 8, 128, 2048, 1 << 30, 4096) < 1 << 40
+
+
 def test_tensors_on_the_host_are_refused():
     x = torch.zeros(2, 64, dtype=BF16)
     with pytest.raises(ValueError, match="device"):
