@@ -10,7 +10,7 @@
 // Scales, the sums of x and the sum over groups are fp32, brought back by 2^12 at the
 // end, and the output is rounded once.  The power of two is what keeps the up to 128
 // products of a sum finite for every finite x (128 * 31 < 2^12); sums below 2^-126
-// lose bits, which takes |x| below 2^-114.
+// lose bits, which takes x or outputs below 2^-114.
 //
 // What bounds it: for wide outputs the codes' stream from HBM, a quarter of the
 // bf16 weights' (1 x 151936 x 4096: 58-64 us, 5.0-5.4 TB/s; a 1 GiB copy reaches

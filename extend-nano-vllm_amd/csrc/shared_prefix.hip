@@ -195,30 +195,35 @@ __device__ __forceinline__ void wide_unit(const AttnParams& p, uint32_t* lds, in
   };
   auto stage = [&](const Tile& t, int b, int key0) {
     uint32_t* base = lds + b * kWideBuf;
-    const int top = key0 + kWideKeys < kv_end ? key0 + kWideKeys - 1 : kv_end - 1;
-    const bool hidden = __any(seen < top);
-    bool bad = false;
-    auto put_v = [&](uint32_t* at, uint4 v) {
-      if (hidden) {
-        const uint4 m = make_uint4(finite_mask(v.x), finite_mask(v.y), finite_mask(v.z), finite_mask(v.w));
-        bad |= (m.x & m.y & m.z & m.w) != 0xFFFFFFFFu;
-        v = make_uint4(v.x & m.x, v.y & m.y, v.z & m.z, v.w & m.w);
-      }
-      *reinterpret_cast<uint4*>(at) = v;
-    };
+    constexpr int kVecs = FP8 ? 2 : 1;                     // staged 16-byte pieces of a granule
+    uint4 v[kPer * kVecs];
 #pragma unroll
     for (int i = 0; i < kPer; ++i) {
       if constexpr (FP8) {
         *reinterpret_cast<bf16x8_t*>(base + kdst[i]) = fp8x8_to_bf16(make_uint2(t.k[i].x, t.k[i].y));
         *reinterpret_cast<bf16x8_t*>(base + kdst[i] + 4) = fp8x8_to_bf16(make_uint2(t.k[i].z, t.k[i].w));
-        put_v(base + vdst[i], __builtin_bit_cast(uint4, fp8x8_to_bf16(make_uint2(t.v[i].x, t.v[i].y))));
-        put_v(base + vdst[i] + 4, __builtin_bit_cast(uint4, fp8x8_to_bf16(make_uint2(t.v[i].z, t.v[i].w))));
+        v[2 * i] = __builtin_bit_cast(uint4, fp8x8_to_bf16(make_uint2(t.v[i].x, t.v[i].y)));
+        v[2 * i + 1] = __builtin_bit_cast(uint4, fp8x8_to_bf16(make_uint2(t.v[i].z, t.v[i].w)));
       } else {
         *reinterpret_cast<uint4*>(base + kdst[i]) = t.k[i];
-        put_v(base + vdst[i], t.v[i]);
+        v[i] = t.v[i];
       }
     }
-    if (bad) last_key[kTileRows] = 1;
+    const int top = key0 + kWideKeys < kv_end ? key0 + kWideKeys - 1 : kv_end - 1;
+    if (__any(seen < top)) {
+      uint32_t all = 0xFFFFFFFFu;
+#pragma unroll
+      for (int i = 0; i < kPer * kVecs; ++i) {
+        const uint4 m = make_uint4(finite_mask(v[i].x), finite_mask(v[i].y), finite_mask(v[i].z),
+                                   finite_mask(v[i].w));
+        all &= m.x & m.y & m.z & m.w;
+        v[i] = make_uint4(v[i].x & m.x, v[i].y & m.y, v[i].z & m.z, v[i].w & m.w);
+      }
+      if (all != 0xFFFFFFFFu) last_key[kTileRows] = 1;
+    }
+#pragma unroll
+    for (int i = 0; i < kPer * kVecs; ++i)
+      *reinterpret_cast<uint4*>(base + vdst[i / kVecs] + 4 * (i % kVecs)) = v[i];
   };
 
   float m_run = -INFINITY, l_run = 0.0f;
