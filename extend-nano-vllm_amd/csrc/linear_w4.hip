@@ -12,12 +12,15 @@
 // products of a sum finite for every finite x (128 * 31 < 2^12); sums below 2^-126
 // lose bits, which takes x or outputs below 2^-114.
 //
-// What bounds it: for wide outputs the codes' stream from HBM, a quarter of the
-// bf16 weights' (1 x 151936 x 4096: 58-64 us, 5.0-5.4 TB/s; a 1 GiB copy reaches
-// 5.07).  Below that the start (at 1 x 4096 x 4096, 5.1 us, x is staged 2.1 us
-// into the kernel's 4.1).  From some dozen rows on a step's work, products, codes
-// to operands, scales and x through LDS, each about a quarter of its time (64 x
-// 24576 x 4096, 37 us: matrix and vector units busy 34% and 31% of the cycles).
+// What bounds it (times of the kernel alone, from a trace): for wide outputs the
+// codes' stream from HBM, a quarter of the bf16 weights' (1 x 151936 x 4096: 65 us,
+// 4.9 TB/s; a 1 GiB copy reaches 5.07).  Below that the launch and the start (1 x
+// 4096 x 4096: 5.6 us, an empty kernel 2.2; a workgroup has its x staged 2.1 us after
+// its first instruction and ends at 4.1).  From some dozen rows on a step's work,
+// products, codes to operands, scales and x through LDS, each about a quarter of its
+// time (64 x 24576 x 4096, 37 us: under counters matrix and vector units are busy 21%
+// and 20% of the cycles, waves wait half of theirs).  Prompts take the slab of 64 rows
+// again and again: 4096 x 24576 x 4096 1.46 ms, 564 TFLOP/s.
 //
 // Codes come to the waves in steps: 256 codes of each of 16 rows, 128 bytes of a
 // row.  A lane's 16 bytes are 32 codes of one row (lane l: row l % 16, codes
@@ -33,8 +36,8 @@
 // (a group's sum of x is a product with ones beside the others).  More rows would
 // leave room for short ranges only, whose staging and joining took most of the time
 // (61 x 6144 x 4096 21.5 us, 64 x 24576 x 4096 45); there x passes through LDS in
-// chunks of 128 (17.7 and 37 us).  For up to 16 rows the chunks are the slower form
-// where N is wide (16 x 24576 x 4096 18.8 us against 17.9).
+// chunks of 128 (17.1 and 37 us).  For up to 16 rows the chunks are the slower form
+// where N is wide (16 x 24576 x 4096 18.8 us against 17.9, timed side by side).
 //
 // Ranges of K shared out over workgroups leave fp32 parts that a second kernel
 // sums in order.
@@ -642,10 +645,10 @@ int32_t device_cus() {
 // before and behind them, and with several ranges the summing kernel.
 //   * Up to 16 rows two workgroups share a CU and its time; a range's x is staged
 //     first, and LDS bounds the range.  Fitted to 18 shapes (1-64 rows, N 800-151936,
-//     K 640-25600, groups of 32-128) timed over all choices, where its choice is 3%
-//     from the best: 1 x 4096 x 4096 one range with eight waves a tile 5.5 us, with
-//     four 7.2, eight ranges with one 7.4; 16 x 5120 x 25600 twelve ranges 23.9, six
-//     24.3, sixteen 25.3.
+//     K 640-25600, groups of 32-128) timed over all choices (the times here are that
+//     sweep's), where its choice is 3% from the best: 1 x 4096 x 4096 one range with
+//     eight waves a tile 5.5 us, with four 7.2, eight ranges with one 7.4; 16 x 5120 x
+//     25600 twelve ranges 23.9, six 24.3, sixteen 25.3.
 //   * More rows take a CU a workgroup; a step costs more where fewer waves share its
 //     x.  Fitted to 17 shapes (17-256 rows, N 1024-151936, K 512-25600), 1% from the
 //     best: 61 x 6144 x 4096 one range with eight waves a tile 17.7 us, two with four

@@ -13,10 +13,11 @@
 // rotation is float32 with one rounding to the tensor's type.
 //
 // What bounds it: memory (each element once in and once out) from some thousand
-// tokens up, launch latency below: 16384 tokens of 40 bf16 heads, 336 MB, 67-74 us
-// (4.6-5.0 TB/s; a copy reaches 5.07), 384 tokens 4.0 us, one token 2.4.  A
-// workgroup takes a token: its threads first form one angle each, shared by all
-// heads through LDS, then turn pairs 16 bytes at a time.
+// tokens up, launch latency below: 16384 tokens of 40 bf16 heads, 336 MB, 67-68 us
+// (5.0 TB/s; a copy reaches 5.07), 384 tokens 4.4 us, one token 2.3.  A workgroup
+// takes a token: its threads first form one angle each, shared by all heads through
+// LDS, then turn pairs 16 bytes at a time.  With few heads that leaves most threads
+// idle: 16384 tokens of one head of 64 elements, 4.2 MB, take 11 us.
 #include <type_traits>
 
 #include "common.h"
